@@ -28,7 +28,10 @@ SOURCES = {
     'drk_train_fused_bf16.hip': ['-ffp-contract=off'],
     'drk_group_bf16.hip': ['-ffp-contract=off'],
 }
-COMMON = ['--offload-arch=gfx950', '-O3', '-fPIC', '-std=c++17', '-Wall', '-Wno-unused-function']
+# The compiler is kept from forming packed fp32 arithmetic (v_pk_add/mul/fma_f32) by itself: some of its forms have given
+# wrong results on this hardware now and then.  (hipcc's host pass says that it does not know the feature: harmless.)
+COMMON = ['--offload-arch=gfx950', '-O3', '-fPIC', '-std=c++17', '-Wall', '-Wno-unused-function',
+          '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 
 
 def _hipcc():
