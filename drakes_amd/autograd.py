@@ -650,3 +650,30 @@ class _SoftStepWideFn(torch.autograd.Function):
 
 def soft_step_wide_with_grad(logits, x_soft, d_t, mc_s, temp, gtemp, mask_index, seed, step, sample_offset, uniforms):
     return _SoftStepWideFn.apply(logits, x_soft, d_t, mc_s, temp, gtemp, mask_index, seed, step, sample_offset, uniforms)
+
+
+class _TokenScoresFn(torch.autograd.Function):
+    """(logp, entropy, top_ids, top_logp) of given tokens; the softmax is recomputed from the logits in the backward."""
+
+    @staticmethod
+    def forward(ctx, logits, tokens, allowed, temp, topk):
+        s = ops.token_scores(logits, tokens, allowed=allowed, temp=temp, topk=topk)
+        ctx.save_for_backward(logits, tokens, allowed, *s)
+        ctx.temp = temp
+        ctx.set_materialize_grads(False)
+        if topk:
+            ctx.mark_non_differentiable(s.top_ids)
+        return s.logp, s.entropy, s.top_ids, s.top_logp
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_logp, g_entropy, _g_ids, g_top):
+        logits, tokens, allowed, *s = ctx.saved_tensors
+        dense = lambda g: None if g is None else g.contiguous()
+        return (ops.token_scores_bwd(logits, tokens, ops.TokenScores(*s), g_logp=dense(g_logp), g_entropy=dense(g_entropy),
+                                     g_top=dense(g_top), allowed=allowed, temp=ctx.temp),) + (None,) * 4
+
+
+def token_scores_with_grad(logits, tokens, *, allowed=None, temp=1.0, topk=0):
+    """ops.token_scores under autograd: -> (logp, entropy, top_ids, top_logp), differentiable in the logits."""
+    return _TokenScoresFn.apply(logits, tokens, allowed, float(temp), topk)

@@ -286,6 +286,23 @@ class Diffusion(nn.Module):
             total += acc.sum(dim=-1)
         return total / n_samples
 
+    def score_tokens(self, x, sigma, targets, *, topk=0, temp=1.0):
+        """What the denoiser says about given tokens: for every position of the (partly masked) x int64 [B, L] or soft state
+        [B, L, 5] at noise level sigma, log p(targets[b, l] | x) over the four nucleotides, the entropy of that
+        distribution and its `topk` most likely nucleotides.  targets int64 [B, L], negative = not scored.
+        -> (logp, entropy, top_ids, top_logp); differentiable: -logp is the masked-token training loss."""
+        from .autograd import token_scores_with_grad
+        sigma = self._process_sigma(sigma)
+        if not self.time_conditioning:
+            sigma = sigma[:1]
+        self.backbone.train_dtype = self._soft_dtype()
+        logits = self.backbone(x, sigma)
+        answers = getattr(self, '_answers', None)
+        if answers is None or answers.device != logits.device:
+            answers = torch.arange(self.vocab_size, device=logits.device) != self.mask_index
+            self._answers = answers
+        return token_scores_with_grad(logits, targets.contiguous(), allowed=answers, temp=temp, topk=topk)
+
     # ------------------------------------------------------------------ fine-tuning sampler
     def _ddpm_update_finetune_gradient(self, x, t, dt, copy_flag_temp, return_process=False, **kw):
         from . import finetune

@@ -4,7 +4,9 @@ PyTorch is plumbing here: it owns device memory and the stream; every op below i
 into libdrakes_hip.so on raw device pointers.  Tensors must live on a ROCm device; nothing
 falls back to torch kernels.
 """
+import collections
 import ctypes
+import math
 
 import torch
 
@@ -606,3 +608,97 @@ def reverse_step_soft_wide_bwd(logits, x_soft, grad_x_next, grad_flag, d_t, move
               mask_index, float(temp), float(d_t), float(move_chance_s), float(gumbel_temp), seed, step, sample_offset,
               _stream())
     return dlogits, dx
+
+
+# ---- scores of given tokens ------------------------------------------------------------------------
+TOPK_MAX = 32
+_SCORE_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+# logp [...], entropy [...] or None, top_ids / top_logp [..., k] or None, stats [..., 2] (what the backward needs)
+TokenScores = collections.namedtuple('TokenScores', 'logp entropy top_ids top_logp stats')
+
+
+def _here(name, *tensors):
+    """Every tensor is on the current device: its stream is the one the launch goes to."""
+    cur = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.is_cuda and t.device.index != cur:
+            raise ValueError(f'{name}: tensor on {t.device}, but the current device is cuda:{cur}')
+
+
+def _row_stride(t, name):
+    """Elements between the rows [..., V] of `t`: the last dimension is contiguous and the leading ones step evenly."""
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f'{name}: the last dimension must be contiguous')
+    stride, rows = None, 1
+    for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if n == 1:
+            continue
+        if stride is None:
+            stride = s
+        elif s != stride * rows:
+            raise ValueError(f'{name}: the rows must lie at even distances')
+        rows *= n
+    return t.shape[-1] if stride is None else stride
+
+
+def _score_args(name, logits, tokens, allowed, temp):
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
+        raise _lib.DrakesHipError(f'{name}: expected logits on the GPU (drakes_amd has no CPU path)')
+    if logits.dtype not in _SCORE_TYPES:
+        raise TypeError(f'{name}: logits are float32, bfloat16 or float16, got {logits.dtype}')
+    if logits.ndim < 1 or logits.shape[-1] < 1 or tuple(tokens.shape) != tuple(logits.shape[:-1]):
+        raise ValueError(f'{name}: logits [..., V] and tokens [...], got {tuple(logits.shape)} and {tuple(tokens.shape)}')
+    if not (0.0 < temp < math.inf):
+        raise ValueError(f'{name}: temp must be positive, got {temp}')
+    V = logits.shape[-1]
+    al, al_stride = None, 0
+    if allowed is not None:
+        if allowed.dtype not in (torch.bool, torch.uint8):
+            raise TypeError(f'{name}: allowed is bool or uint8, got {allowed.dtype}')
+        if tuple(allowed.shape) not in ((V,), tuple(logits.shape)):
+            raise ValueError(f'{name}: allowed has shape [V] or that of the logits, got {tuple(allowed.shape)}')
+        al, al_stride = _dev_ptr(allowed, allowed.dtype, 'allowed'), V if allowed.ndim > 1 or logits.ndim == 1 else 0
+    _here(name, logits, tokens, allowed)
+    return (ctypes.c_void_p(logits.data_ptr()), _SCORE_TYPES[logits.dtype], _row_stride(logits, name), _i(tokens, 'tokens'), al,
+            al_stride, float(temp))
+
+
+def token_scores(logits, tokens, *, allowed=None, temp=1.0, topk=0, entropy=True):
+    """Log-probability of each given token, the row's entropy and its `topk` most likely tokens (drk_token_scores).
+
+    logits [..., V] float32 / bfloat16 / float16 (a slice of wider rows will do), tokens int64 [...]: negative = not
+    scored; allowed: bool / uint8 [V] or [..., V], the columns that count.  -> TokenScores, float32."""
+    args = _score_args('token_scores', logits, tokens, allowed, temp)
+    V = logits.shape[-1]
+    if not 0 <= topk <= min(V, TOPK_MAX):
+        raise ValueError(f'token_scores: topk must be in [0, min(V, {TOPK_MAX})], got {topk}')
+    new = lambda *last, dtype=torch.float32: torch.empty(*tokens.shape, *last, dtype=dtype, device=logits.device)
+    s = TokenScores(new(), new() if entropy else None, new(topk, dtype=torch.int64) if topk else None,
+                    new(topk) if topk else None, new(2))
+    _lib.call('drk_token_scores', *args, topk, _raw(s.logp), _raw(s.entropy), _raw(s.top_ids), _raw(s.top_logp), _raw(s.stats),
+              tokens.numel(), V, _stream())
+    return s
+
+
+def token_scores_bwd(logits, tokens, scores, *, g_logp=None, g_entropy=None, g_top=None, allowed=None, temp=1.0, out=None):
+    """dlogits (dense, of the logits' type) from the gradients of logp, entropy and top_logp (drk_token_scores_bwd);
+    `scores`: what token_scores gave for the same arguments.  out: dense; it may be the logits themselves."""
+    args = _score_args('token_scores_bwd', logits, tokens, allowed, temp)
+    V = logits.shape[-1]
+    shape = tuple(tokens.shape)
+    if g_entropy is not None and scores.entropy is None:
+        raise ValueError('token_scores_bwd: g_entropy needs the entropy')
+    if g_top is not None and scores.top_ids is None:
+        raise ValueError('token_scores_bwd: g_top needs the top alternatives')
+    k = scores.top_ids.shape[-1] if g_top is not None else 0
+    for t, want, name in ((g_logp, shape, 'g_logp'), (g_entropy, shape, 'g_entropy'), (g_top, shape + (k,), 'g_top'),
+                          (scores.stats, shape + (2,), 'stats'), (out, tuple(logits.shape), 'out')):
+        if t is not None and tuple(t.shape) != want:
+            raise ValueError(f'token_scores_bwd: {name} has shape {want}, got {tuple(t.shape)}')
+    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if out is None else out
+    _here('token_scores_bwd', g_logp, g_entropy, g_top, scores.stats, out)
+    _lib.call('drk_token_scores_bwd', *args, k, _f(scores.stats, 'stats'), _f(scores.entropy, 'entropy') if g_entropy is not None else None,
+              _i(scores.top_ids, 'top_ids') if k else None, _f(g_logp, 'g_logp'), _f(g_entropy, 'g_entropy'), _f(g_top, 'g_top'),
+              _dev_ptr(out, logits.dtype, 'out'), tokens.numel(), V, _stream())
+    return out

@@ -62,6 +62,18 @@ class Interpolant:
             t_1 = t_2
         return pred, prot_traj, clean_traj
 
+    def score_tokens(self, model, X, aatypes, targets, mask, chain_M, residue_idx, chain_encoding_all, *, topk=0, allowed=None):
+        """What the denoiser says about given residues: log p(targets[b, l] | aatypes) at the sampler's temperature, the
+        entropy and the `topk` most likely residues, at every position of the (partly masked) aatypes int64 [B, L].
+        Positions outside `mask` and negative targets are not scored; the mask token is no answer; allowed: bool [22] or
+        [B, L, 22], what else may stand there.  -> (logp, entropy, top_ids, top_logp), differentiable in the model."""
+        logits = model(X, aatypes, mask, chain_M, residue_idx, chain_encoding_all)
+        answers = torch.arange(self.num_tokens, device=logits.device) != MASK_TOKEN_INDEX
+        if allowed is not None:
+            answers = (answers & allowed).contiguous()
+        targets = torch.where(mask != 0, targets, torch.full_like(targets, -1))
+        return autograd.token_scores_with_grad(logits, targets, allowed=answers, temp=float(self._cfg.temp), topk=topk)
+
     def sample_gradient(self, model, X, mask, chain_M, residue_idx, chain_encoding_all, truncate_steps, gumbel_softmax_temp,
                         *, seed=None, sample_offset=0, uniforms=None):
         """Reference signature and return value (:142-209): (straight-through one-hot sample [B,L,22] with grad,

@@ -109,6 +109,35 @@ int drk_q_xt(const int64_t* x0, const float* uniforms, int64_t* xt, int B, int L
 int drk_likelihood_accum(const float* logits, const int64_t* x0, const int64_t* xt, float multiplier, float* acc,
                          int B, int L, void* stream);
 
+/* ---- scores of given tokens: log-probability, entropy, top alternatives, any vocabulary --------------------------
+ * logits: rows of V values of type `dtype`, row r at logits + r * row_stride values (row_stride 0: one row for all);
+ * tokens int64 [rows].  A column counts when allowed is NULL or allowed[r * allowed_stride + j] != 0 (uint8;
+ * allowed_stride 0: one list for all rows, else >= V) and its logit is not -inf; what stands in other columns is never
+ * looked at.  With p = softmax over those columns of logits / temp (0 < temp < inf):
+ *   logp [rows]: log p(token); 0 for a negative token (not scored), -inf for a column that does not count, NaN for a
+ *                token >= V;
+ *   entropy [rows] (optional): -sum p log p, in nats;
+ *   top_ids int64, top_logp [rows][k]: the k largest, equal logits by the lower index; -1 and -inf where fewer count.
+ *                0 <= k <= min(V, DRK_TOPK_MAX);
+ *   stats [rows][2]: (largest logit, log of the sum of exp((logit - largest) / temp)): drk_token_scores_bwd's input.
+ * A row in which no column counts has entropy 0, logp -inf and ids -1; a NaN or +inf in a column that counts makes the
+ * row's logp, entropy and top_logp NaN.  All results float32. */
+#define DRK_F32 0
+#define DRK_BF16 1
+#define DRK_F16 2
+#define DRK_TOPK_MAX 32
+int drk_token_scores(const void* logits, int dtype, long row_stride, const int64_t* tokens, const unsigned char* allowed,
+                     long allowed_stride, float temp, int k, float* logp, float* entropy, int64_t* top_ids,
+                     float* top_logp, float* stats, long rows, int V, void* stream);
+/* Gradient of sum g_logp logp + sum g_entropy entropy + sum g_top top_logp with respect to the logits (each g optional;
+ * g_entropy needs the entropy, g_top the ids that the forward gave, else k = 0).  dlogits [rows][V], dense, of the logits'
+ * type, every element written: 0 in columns that do not count; it may be the logits themselves when they are dense.  A log-probability of -inf, 0 (not scored) or NaN (token
+ * >= V) passes no gradient, nor does a place with id -1. */
+int drk_token_scores_bwd(const void* logits, int dtype, long row_stride, const int64_t* tokens, const unsigned char* allowed,
+                         long allowed_stride, float temp, int k, const float* stats, const float* entropy,
+                         const int64_t* top_ids, const float* g_logp, const float* g_entropy, const float* g_top,
+                         void* dlogits, long rows, int V, void* stream);
+
 /* ---- denoiser (CNNModel.forward, models/dnaconv.py:74-110), fp32 ---------------------------- */
 /* relu(Linear(GaussianFourierProjection(sigma))) — dnaconv.py:19-21,50,82.
  * sigma [nb]; W [64]; lin_w [128][128]; lin_b [128]; temb [nb][128]. */
