@@ -60,6 +60,10 @@ SIGNATURES = {
     'drk_stem_ln_bf16': [_P, _P, _P, _P, c_long, _P, _P, _P, _P, _P, _P, c_int, c_int, _P],
     'drk_gate_bf16': [_P, _P, _P, _P, _P, c_int, c_int, _P, c_long, _P],
     'drk_conv_wgrad_bf16': [_P, _P, _P, c_int, c_int, c_int, c_int, _P, c_long, _P],
+    'drk_ln_fwd_ck8': [_P, _P, c_long, _P, _P, _P, c_int, _P, _P, _P, _P, _P, c_int, c_int, c_int, _P],
+    'drk_ck8_unpack': [_P, _P, _P, c_int, c_int, c_int, _P],
+    'drk_ln_bwd_ck8': [_P] * 11 + [c_int, c_int, _P, c_long, _P],
+    'drk_conv_wgrad_ck8': [_P] * 6 + [c_int, c_int, c_int, c_int, _P, c_long, _P],
     'drk_layer_bwd_bf16': [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_long, c_int, c_int, c_int, c_int, c_int, _P],
     'drk_head_bwd_bf16': [_P, _P, _P, _P, _P, c_long, c_int, c_int, _P],
     'drk_conv_wgrad_bf16_multi': [_P, _P, c_int, _P, c_int, c_int, c_int, c_int, _P, c_long, _P],
@@ -79,6 +83,8 @@ HOST_QUERIES = {
     'drk_conv_wgrad_workspace_bytes': [c_int, c_int, c_int],
     'drk_conv_wgrad_bf16_workspace_bytes': [c_int, c_int, c_int],
     'drk_gate_bf16_workspace_bytes': [],
+    'drk_ln_bwd_ck8_workspace_bytes': [c_int, c_int],
+    'drk_conv_wgrad_ck8_workspace_bytes': [c_int, c_int, c_int],
     'drk_conv_wgrad_bf16_multi_workspace_bytes': [c_int, c_int, c_int, c_int],
     'drk_head_bwd_bf16_slab_floats': [],
     'drk_denoiser_bwd_bf16_slab_floats': [c_int],

@@ -27,6 +27,7 @@ SOURCES = {
     'drk_train_chain.hip': ['-ffp-contract=off'],
     'drk_train_fused_bf16.hip': ['-ffp-contract=off'],
     'drk_group_bf16.hip': ['-ffp-contract=off'],
+    'drk_ck8.hip': ['-ffp-contract=off'],
     'drk_token_scores.hip': ['-ffp-contract=off'],
 }
 # The compiler is kept from forming packed fp32 arithmetic (v_pk_add/mul/fma_f32) by itself: some of its forms have given

@@ -620,10 +620,13 @@ TokenScores = collections.namedtuple('TokenScores', 'logp entropy top_ids top_lo
 
 def _here(name, *tensors):
     """Every tensor is on the current device: its stream is the one the launch goes to."""
-    cur = torch.cuda.current_device()
     for t in tensors:
-        if t is not None and t.is_cuda and t.device.index != cur:
-            raise ValueError(f'{name}: tensor on {t.device}, but the current device is cuda:{cur}')
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise _lib.DrakesHipError(f'{name}: expected tensors on the GPU (drakes_amd has no CPU path)')
+        if t.device.index != torch.cuda.current_device():
+            raise ValueError(f'{name}: tensor on {t.device}, but the current device is cuda:{torch.cuda.current_device()}')
 
 
 def _row_stride(t, name):
@@ -702,3 +705,138 @@ def token_scores_bwd(logits, tokens, scores, *, g_logp=None, g_entropy=None, g_t
               _i(scores.top_ids, 'top_ids') if k else None, _f(g_logp, 'g_logp'), _f(g_entropy, 'g_entropy'), _f(g_top, 'g_top'),
               _dev_ptr(out, logits.dtype, 'out'), tokens.numel(), V, _stream())
     return out
+
+
+# ---- activation checkpoints in 8 bits --------------------------------------------------------------
+# codes int8 [B,L,128], exps uint8 [B,L,4], rstd float32 [B,L] (None without a LayerNorm), gates uint8 [B,L,16] or None;
+# include/drakes_hip.h says what the bytes stand for
+Checkpoint8 = collections.namedtuple('Checkpoint8', 'codes exps rstd gates')
+
+
+def _rows128(t, name):
+    if not isinstance(t, torch.Tensor) or t.ndim != 3 or t.shape[-1] != C:
+        raise ValueError(f'{name}: expected a tensor [B, L, {C}]')
+    return t.shape[0], t.shape[1]
+
+
+def _shaped(t, shape, name):
+    if t is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f'{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}')
+    return t
+
+
+def _ck8(ck, B, L, name, rstd=False):
+    _shaped(ck.codes, (B, L, C), f'{name}: codes'), _shaped(ck.exps, (B, L, C // 32), f'{name}: exps')
+    _shaped(ck.rstd, (B, L), f'{name}: rstd'), _shaped(ck.gates, (B, L, C // 8), f'{name}: gates')
+    if rstd and ck.rstd is None:
+        raise ValueError(f'{name}: the checkpoint was kept without a LayerNorm (rstd is None)')
+    _here(name, ck.codes, ck.exps, ck.rstd, ck.gates)
+    return _dev_ptr(ck.codes, torch.int8, 'codes'), _dev_ptr(ck.exps, torch.uint8, 'exps')
+
+
+def _scratch(nbytes, device):
+    """A workspace of this call's own: freed and reused in stream order by torch's allocator, and kept by a graph that
+    captures the call."""
+    return torch.empty(max(1, nbytes // 4), dtype=torch.float32, device=device)
+
+
+def ln_fwd_ck8(feat, tbias_layer, tb_stride, gamma, beta, *, out=None, relu_mask=None, gate_self=False):
+    """(h, Checkpoint8) of feat float32 [B,L,128]: h = bf16(LayerNorm(feat + tbias) * gamma + beta) and its normalised input
+    kept in 8 bits; gamma None: no LayerNorm, h = bf16(feat) and feat itself is kept.  Gates as bits: from relu_mask uint8
+    [B,L,128], or (gate_self) from feat > 0.  tbias_layer, tb_stride: as for ln_fwd_bf16."""
+    B, L = _rows128(feat, 'ln_fwd_ck8')
+    if (gamma is None) != (beta is None) or (gamma is None and tbias_layer is not None):
+        raise ValueError('ln_fwd_ck8: gamma and beta come together, and tbias needs them')
+    if relu_mask is not None and gate_self:
+        raise ValueError('ln_fwd_ck8: gates come from relu_mask or from feat, not from both')
+    _shaped(relu_mask, (B, L, C), 'ln_fwd_ck8: relu_mask'), _shaped(out, (B, L, C), 'ln_fwd_ck8: out')
+    _shaped(gamma, (C,), 'ln_fwd_ck8: gamma'), _shaped(beta, (C,), 'ln_fwd_ck8: beta')
+    if tbias_layer is not None:
+        if tbias_layer.dtype != torch.float32 or not tbias_layer.is_cuda or tbias_layer.stride(-1) != 1:
+            raise ValueError('ln_fwd_ck8: tbias is float32 on the GPU, contiguous over its channels')
+        # the last row read starts (B - 1) * tb_stride elements behind the first
+        held = tbias_layer.untyped_storage().nbytes() // 4 - tbias_layer.storage_offset()
+        if tb_stride < 0 or max(B - 1, 0) * tb_stride + C > held:
+            raise ValueError('ln_fwd_ck8: tbias does not hold a row for every sequence at this tb_stride')
+    _here('ln_fwd_ck8', feat, tbias_layer, gamma, beta, relu_mask, out)
+    new = lambda n, dt: torch.empty(B, L, n, dtype=dt, device=feat.device)
+    out = new(C, torch.bfloat16) if out is None else out
+    ck = Checkpoint8(new(C, torch.int8), new(C // 32, torch.uint8),
+                     torch.empty(B, L, dtype=torch.float32, device=feat.device) if gamma is not None else None,
+                     new(C // 8, torch.uint8) if relu_mask is not None or gate_self else None)
+    _lib.call('drk_ln_fwd_ck8', _f(feat, 'feat'), _raw(tbias_layer), tb_stride, _f(gamma, 'gamma'), _f(beta, 'beta'),
+              _dev_ptr(relu_mask, torch.uint8, 'relu_mask'), int(gate_self), _b16(out, 'h'), _raw(ck.codes), _raw(ck.exps),
+              _raw(ck.rstd), _raw(ck.gates), B, L, int(gamma is not None), _stream())
+    return out, ck
+
+
+def ck8_unpack(ck, dtype=torch.float32, out=None):
+    """The values a checkpoint stands for, [B,L,128] float32 or bfloat16 (exact in both)."""
+    if out is not None:
+        dtype = out.dtype
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f'ck8_unpack: float32 or bfloat16, got {dtype}')
+    B, L = _rows128(ck.codes, 'ck8_unpack')
+    codes, exps = _ck8(ck, B, L, 'ck8_unpack')
+    out = torch.empty(B, L, C, dtype=dtype, device=ck.codes.device) if out is None else _shaped(out, (B, L, C), 'ck8_unpack: out')
+    _here('ck8_unpack', out)
+    _lib.call('drk_ck8_unpack', codes, exps, _dev_ptr(out, dtype, 'out'), _SCORE_TYPES[dtype], B, L, _stream())
+    return out
+
+
+def ln_bwd_ck8(dh, ck, gamma, g_resid, *, dfeat=None, dxin=None, sums=None, hand_over=True):
+    """(dfeat, dc): LayerNorm backward from a checkpoint, plus g_resid (optional): dfeat float32 [B,L,128] = dL/dfeat, and
+    with hand_over dc = bf16(dfeat * gate), the output gradient of the convolution below.  hand_over False: dc is None and
+    dfeat comes gated if the checkpoint has gates.  dfeat may be dh or g_resid; dxin: receives dL/d(LayerNorm input);
+    sums float32 [4,128] += (dgamma, dbeta, dtime_bias, column sums of the gated dfeat)."""
+    B, L = _rows128(dh, 'ln_bwd_ck8')
+    codes, exps = _ck8(ck, B, L, 'ln_bwd_ck8', rstd=True)
+    _shaped(gamma, (C,), 'ln_bwd_ck8: gamma'), _shaped(sums, (4, C), 'ln_bwd_ck8: sums')
+    for t, name in ((g_resid, 'g_resid'), (dfeat, 'dfeat'), (dxin, 'dxin')):
+        _shaped(t, (B, L, C), f'ln_bwd_ck8: {name}')
+    if hand_over and ck.gates is None:
+        raise ValueError('ln_bwd_ck8: the checkpoint has no gates to hand over')
+    _here('ln_bwd_ck8', dh, gamma, g_resid, dfeat, dxin, sums)
+    dfeat = torch.empty_like(dh) if dfeat is None else dfeat
+    dc = torch.empty(B, L, C, dtype=torch.bfloat16, device=dh.device) if hand_over else None
+    need = _lib.load().drk_ln_bwd_ck8_workspace_bytes(B, L) if sums is not None else 0
+    ws = _scratch(need, dh.device) if need else None
+    _lib.call('drk_ln_bwd_ck8', _f(dh, 'dh'), codes, exps, _f(ck.rstd, 'rstd'), _f(gamma, 'gamma'), _f(g_resid, 'g_resid'),
+              _dev_ptr(ck.gates, torch.uint8, 'gates'), _f(dfeat, 'dfeat'), _raw(dc), _f(dxin, 'dxin'), _f(sums, 'sums'), B, L,
+              _raw(ws), need, _stream())
+    return dfeat, dc
+
+
+def gate_ck8(g, gates, *, colsum=None):
+    """dc = bf16(g * gate) of g float32 [B,L,128] with a checkpoint's gate bits; colsum [128] += column sums of g * gate."""
+    B, L = _rows128(g, 'gate_ck8')
+    _shaped(gates, (B, L, C // 8), 'gate_ck8: gates'), _shaped(colsum, (C,), 'gate_ck8: colsum')
+    _here('gate_ck8', g, gates, colsum)
+    dc = torch.empty(B, L, C, dtype=torch.bfloat16, device=g.device)
+    sums = torch.zeros(4, C, dtype=torch.float32, device=g.device) if colsum is not None else None
+    need = _lib.load().drk_ln_bwd_ck8_workspace_bytes(B, L) if sums is not None else 0
+    ws = _scratch(need, g.device) if need else None
+    _lib.call('drk_ln_bwd_ck8', _f(g, 'g'), None, None, None, None, None, _dev_ptr(gates, torch.uint8, 'gates'), None, _raw(dc),
+              None, _raw(sums), B, L, _raw(ws), need, _stream())
+    if colsum is not None:
+        colsum += sums[3]
+    return dc
+
+
+def conv_wgrad_ck8(ck, gamma, beta, dc, dwt, dilation):
+    """dwt float32 [taps,128(ci),128(co)] += sum_rows h[row + off][ci] * dc[row][co], h = gamma * xq + beta of a checkpoint
+    (gamma, beta None: h = xq), dc bf16 [B,L,128]; exact products, fp32 sums in a fixed order."""
+    B, L = _rows128(dc, 'conv_wgrad_ck8')
+    codes, exps = _ck8(ck, B, L, 'conv_wgrad_ck8')
+    if (gamma is None) != (beta is None):
+        raise ValueError('conv_wgrad_ck8: gamma and beta come together')
+    _shaped(gamma, (C,), 'conv_wgrad_ck8: gamma'), _shaped(beta, (C,), 'conv_wgrad_ck8: beta')
+    taps = dwt.shape[0]
+    _shaped(dwt, (taps, C, C), 'conv_wgrad_ck8: dwt')
+    if not (1 <= taps <= 9 and taps % 2 == 1) or dilation < 0:
+        raise ValueError(f'conv_wgrad_ck8: an odd number of taps up to 9 and dilation >= 0, got {taps}, {dilation}')
+    _here('conv_wgrad_ck8', gamma, beta, dc, dwt)
+    need = _lib.load().drk_conv_wgrad_ck8_workspace_bytes(B, L, taps)
+    ws = _scratch(need, dc.device)
+    _lib.call('drk_conv_wgrad_ck8', codes, exps, _f(gamma, 'gamma'), _f(beta, 'beta'), _b16(dc, 'dc'), _f(dwt, 'dwt'), B, L, taps,
+              dilation, _raw(ws), need, _stream())

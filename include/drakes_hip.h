@@ -366,6 +366,41 @@ long drk_conv_wgrad_bf16_workspace_bytes(int B, int L, int taps);
 int drk_conv_wgrad_bf16(const void* h, const void* dc, float* dwt, int B, int L, int taps, int dilation, void* workspace,
                         long workspace_bytes, void* stream);
 
+/* ---- activation checkpoints in 8 bits --------------------------------------------------------------------------------
+ * A checkpoint of B*L rows of 128 channels (the same models/dnaconv.py:88-101 layers as above, kept for a backward pass):
+ *   codes int8 [B*L][128], exps uint8 [B*L][4]: channel c is codes[c] * 2^(exps[c / 32] - 127); a block of 32 channels has
+ *     the smallest power of two that keeps it within +-127 steps (at least 2^-126), codes rounded to nearest, ties to even.
+ *     exps 0: all zero; 255: the block held an infinity, a NaN or a magnitude above 127 * 2^120, and reads back as NaN;
+ *   rstd float32 [B*L]: the LayerNorm's 1 / sqrt(var + 1e-5);
+ *   gates uint8 [B*L][16]: bit c % 8 of byte c / 8 = the ReLU below was open at channel c. */
+/* ln = 1: x^ = (feat + tbias - mean) * rstd is what the checkpoint holds, h = bf16(x^ * gamma + beta); statistics and codes
+ * in fp64.  ln = 0: the checkpoint holds feat itself, h = bf16(feat); tbias, gamma, beta, rstd NULL.  tbias as for
+ * drk_ln_fwd_bf16 (tb_stride a multiple of 4).  gates: from relu_mask uint8 [B*L][128] (non-zero = open), from feat > 0
+ * (gate_self = 1), or NULL.  feat, h, tbias, gamma, beta 16-byte aligned, codes and relu_mask 8-byte. */
+int drk_ln_fwd_ck8(const float* feat, const float* tbias, long tb_stride, const float* gamma, const float* beta,
+                   const unsigned char* relu_mask, int gate_self, void* h, signed char* codes, unsigned char* exps,
+                   float* rstd, unsigned char* gates, int B, int L, int ln, void* stream);
+/* The values a checkpoint stands for, [B*L][128] float32 (dtype DRK_F32) or bf16 (DRK_BF16); both are exact. */
+int drk_ck8_unpack(const signed char* codes, const unsigned char* exps, void* out, int dtype, int B, int L, void* stream);
+/* LayerNorm backward from a checkpoint, with the residual add and the gate of the layer below:
+ *   a = dh * gamma;  dx = rstd * (a - mean_c(a) - xq * mean_c(a * xq))     (codes NULL: no LayerNorm, dx = dh)
+ *   d = dx + g_resid (NULL: + 0);  dfeat = d, dc = bf16(d * gate);  with gates and no dc: dfeat = d * gate
+ * dh, g_resid, dfeat (optional beside dc), dxin (optional: dx) float32 [B*L][128]; dc bf16 [B*L][128].  dfeat may be dh or
+ * g_resid.  sums (optional) float32 [4][128] += column sums of dh * xq (dgamma), dh (dbeta), dx (the time bias), d * gate (the
+ * lower convolution's bias; gates NULL: d), in a fixed order through `workspace` (drk_ln_bwd_ck8_workspace_bytes(B, L)
+ * bytes); without a LayerNorm the first two stay as they are.  All pointers 16-byte aligned, codes 8. */
+long drk_ln_bwd_ck8_workspace_bytes(int B, int L);
+int drk_ln_bwd_ck8(const float* dh, const signed char* codes, const unsigned char* exps, const float* rstd,
+                   const float* gamma, const float* g_resid, const unsigned char* gates, float* dfeat, void* dc, float* dxin,
+                   float* sums, int B, int L, void* workspace, long workspace_bytes, void* stream);
+/* drk_conv_wgrad_bf16 with the checkpoint in the place of h: dwt[t][ci][co] += sum_rows h[row + (t - taps/2)*dilation][ci] *
+ * dc[row][co], h = gamma * xq + beta (gamma, beta NULL: h = xq) and 0 outside the row's sequence; taps odd, <= 9.  Exact
+ * products, fp32 sums in a fixed order. */
+long drk_conv_wgrad_ck8_workspace_bytes(int B, int L, int taps);
+int drk_conv_wgrad_ck8(const signed char* codes, const unsigned char* exps, const float* gamma, const float* beta,
+                       const void* dc, float* dwt, int B, int L, int taps, int dilation, void* workspace,
+                       long workspace_bytes, void* stream);
+
 /* ---- round 3: the bf16 backward as ONE launch per layer, parameter gradients deferred -------------------------------
  * (reference: torch autograd over models/dnaconv.py:88-101 inside the K Gumbel-softmax steps of
  * _sample_finetune_gradient, diffusion_gosai_update.py:589-630; the optimizer reads the gradients only after the whole
