@@ -29,8 +29,8 @@ SIGNATURES = {
     'drk_denoise_argmax': [_P, _P, _P, c_int, c_int, _P],
     'drk_q_xt': [_P, _P, _P, c_int, c_int, c_float, _P, c_uint64, c_uint32, c_uint64, _P],
     'drk_likelihood_accum': [_P, _P, _P, c_float, _P, c_int, c_int, _P],
-    'drk_token_scores': [_P, c_int, c_long, _P, _P, c_long, c_float, c_int, _P, _P, _P, _P, _P, c_long, c_int, _P],
-    'drk_token_scores_bwd': [_P, c_int, c_long, _P, _P, c_long, c_float, c_int, _P, _P, _P, _P, _P, _P, _P, c_long, c_int, _P],
+    'drk_token_scores': [_P, c_int, c_long, _P, _P, c_long, c_float, c_int, _P, _P, _P, _P, _P, c_long, c_int, _P, c_long, _P],
+    'drk_token_scores_bwd': [_P, c_int, c_long, _P, _P, c_long, c_float, c_int, _P, _P, _P, _P, _P, _P, _P, _P, c_long, c_int, _P],
     'drk_time_embed_fwd': [_P, c_int, _P, _P, _P, _P, _P],
     'drk_time_bias_fwd': [_P, c_int, _P, _P, c_int, _P, _P],
     'drk_stem_fwd': [_P, _P, _P, _P, _P, c_int, c_int, _P],
@@ -83,6 +83,7 @@ HOST_QUERIES = {
     'drk_conv_wgrad_workspace_bytes': [c_int, c_int, c_int],
     'drk_conv_wgrad_bf16_workspace_bytes': [c_int, c_int, c_int],
     'drk_gate_bf16_workspace_bytes': [],
+    'drk_token_scores_workspace_bytes': [c_long, c_int, c_int],
     'drk_ln_bwd_ck8_workspace_bytes': [c_int, c_int],
     'drk_conv_wgrad_ck8_workspace_bytes': [c_int, c_int, c_int],
     'drk_conv_wgrad_bf16_multi_workspace_bytes': [c_int, c_int, c_int, c_int],

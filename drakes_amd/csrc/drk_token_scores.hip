@@ -10,27 +10,38 @@
 // Sums are fp32 over partial sums of a thread's own elements, joined in a fixed order: results are reproducible.
 // Where exp((x - m) / T) is 0, x - m may be -inf (the difference of a type's lowest value overflows); as a factor it is
 // held at -1e20, so that the product is 0 and not NaN.  A NaN or +inf among A makes s, logp and H NaN.
+//
+// A forward pass reads every logit once (the bound: HBM), a backward pass reads them again and writes as much.  Three
+// shapes of work, chosen by V and the number of rows alone:
+//   V <= 64        one thread per row; 64 rows at a time come through LDS, so that short rows are still read and written as
+//                  whole cache lines (k_scores_small, k_scores_small_bwd);
+//   longer rows    one wave (up to 256 16-byte pieces) or four waves per row, one pass with a running maximum, sum and
+//                  entropy sum per thread (k_scores_row, k_scores_row_bwd);
+//   few long rows  a row is split over workgroups, whose partial results a second launch joins in order (k_scores_join).
+// Top alternatives without a second pass over the row: every thread has the maximum of its own elements; the k-th largest
+// of a wave's 64 maxima is a lower bound of the row's k-th largest element, so only threads whose maximum reaches the
+// largest such bound can hold an alternative.  Their elements are read again (a few hundred per row), those above the bound
+// are listed, and the k that fewest others precede are the answer.  A row with more equal elements at the bound than the
+// list holds (a constant row) is searched k times instead.
 #include "drk_common.h"
 #include "../../include/drakes_hip.h"
 
 #define TSCHECK(cond, name) \
   if (!(cond)) return drk_set_error_msg(DRK_EINVAL, name ": bad arguments")
 
-#define TS_THREADS 256
-
 struct ts_f32 {
   typedef float T;
-  static __device__ __forceinline__ float get(const T* p) { return *p; }
+  static __device__ __forceinline__ float get(T v) { return v; }
   static __device__ __forceinline__ T put(float v) { return v; }
 };
 struct ts_bf16 {
   typedef __bf16 T;
-  static __device__ __forceinline__ float get(const T* p) { return (float)*p; }
+  static __device__ __forceinline__ float get(T v) { return (float)v; }
   static __device__ __forceinline__ T put(float v) { return (__bf16)v; }
 };
 struct ts_f16 {
   typedef _Float16 T;
-  static __device__ __forceinline__ float get(const T* p) { return (float)*p; }
+  static __device__ __forceinline__ float get(T v) { return (float)v; }
   static __device__ __forceinline__ T put(float v) { return (_Float16)v; }
 };
 
@@ -53,93 +64,123 @@ __device__ __forceinline__ ts_acc ts_join(ts_acc a, ts_acc b, float c) {
   o.t = (a.t + a.s * ts_factor(da)) * fa + (b.t + b.s * ts_factor(db)) * fb;
   return o;
 }
+__device__ __forceinline__ ts_acc ts_join_wave(ts_acc v, float c) {
+#pragma unroll
+  for (int w = 32; w > 0; w >>= 1) {
+    const ts_acc o = {__shfl_xor(v.m, w), __shfl_xor(v.s, w), __shfl_xor(v.t, w)};
+    v = ts_join(v, o, c);
+  }
+  return v;
+}
 
 struct TsArgs {
   const void* x;
   const int64_t* tok;
   const unsigned char* allowed;
-  long allowed_stride, row_stride;
+  long allowed_stride, row_stride, rows;
   float *logp, *entropy, *stats, *top_logp;
   int64_t* top_ids;
-  int V, k;
+  void* parts;                 // split rows: [rows][splits] TsPart
+  int V, k, splits, per_part;  // per_part: 16-byte pieces of a part
   float inv_temp;
 };
+struct TsPart {                // partial result of a part of a row: 16 + 8 * DRK_TOPK_MAX bytes
+  ts_acc v;
+  int n;
+  float x[DRK_TOPK_MAX];
+  int at[DRK_TOPK_MAX];
+};
 
-// A row's written results, by one thread: x_t is read again.
-template <class D>
-__device__ __forceinline__ void ts_finish(const TsArgs& a, long row, ts_acc v) {
-  const typename D::T* x = (const typename D::T*)a.x + row * a.row_stride;
-  const unsigned char* al = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
-  const float ls = v.s == 0.f ? 0.f : logf(v.s);
-  a.stats[2 * row] = v.m;
-  a.stats[2 * row + 1] = ls;
+__device__ __forceinline__ float ts_logp(float x, ts_acc v, float ls, float inv_temp) {
+  return v.s != v.s ? NAN : (x - v.m) * inv_temp - ls;
+}
+__device__ __forceinline__ float ts_log_sum(ts_acc v) { return v.s == 0.f ? 0.f : logf(v.s); }
+
+// A row's scalars, by one thread; xt: the given token's logit, -inf where its column does not count.
+__device__ __forceinline__ void ts_finish(const TsArgs& a, long row, ts_acc v, float ls, int64_t t, float xt) {
+  *(float2*)(a.stats + 2 * row) = make_float2(v.m, ls);
   if (a.entropy) a.entropy[row] = v.s == 0.f ? 0.f : ls - a.inv_temp * (v.t / v.s);
-  const int64_t t = a.tok[row];
-  float lp = 0.f;
-  if (t >= a.V) {
-    lp = NAN;
-  } else if (t >= 0) {
-    const float xt = D::get(x + t);
-    const bool in = (!al || al[t]) && xt != -INFINITY;
-    lp = v.s != v.s ? NAN : in ? (xt - v.m) * a.inv_temp - ls : -INFINITY;
-  }
-  a.logp[row] = lp;
+  a.logp[row] = t < 0 ? 0.f : t >= a.V ? NAN : xt == -INFINITY ? (v.s != v.s ? NAN : -INFINITY) : ts_logp(xt, v, ls, a.inv_temp);
+}
+template <class D>
+__device__ __forceinline__ float ts_token(const TsArgs& a, long row, int64_t t) {
+  if (t < 0 || t >= a.V || (a.allowed && !a.allowed[row * a.allowed_stride + t])) return -INFINITY;
+  return D::get(((const typename D::T*)a.x)[row * a.row_stride + t]);
 }
 
-template <class D>
-__global__ void __launch_bounds__(TS_THREADS) k_token_scores(TsArgs a) {
-  __shared__ ts_acc red[TS_THREADS];
-  __shared__ float bv[TS_THREADS];
-  __shared__ int bi[TS_THREADS];
-  const long row = blockIdx.x;
-  const int tid = threadIdx.x;
-  const typename D::T* x = (const typename D::T*)a.x + row * a.row_stride;
-  const unsigned char* al = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
+// ---------------------------------------------------------------------------------------------- V <= 64: a thread per row
+#define TS_SMALL_V 64
+// a row's word j in LDS: one pad word after every 64, so that 64 threads at a stride of V words meet few banks twice
+__device__ __forceinline__ int ts_pad(int i) { return i + (i >> 6); }
+#define TS_SMALL_LDS (TS_SMALL_V * 64 + TS_SMALL_V)
+
+// n consecutive rows -> LDS as floats, -inf in columns that a per-row list leaves out.  VEC: the rows are dense and 16-byte
+// aligned (and so is the list, by its own width): whole 16-byte pieces.
+template <class D, bool VEC>
+__device__ __forceinline__ void ts_stage(const typename D::T* x, const unsigned char* al, long row_stride, int V, int n, float* lds) {
+  constexpr int E = 16 / sizeof(typename D::T);
+  const int lane = threadIdx.x, total = n * V;
+  if (VEC) {
+    struct alignas(16) piece { typename D::T v[E]; };
+    struct alignas(E) bytes { unsigned char v[E]; };
+    const int whole = total / E;
+    for (int i = lane; i < whole; i += 64) {
+      const piece p = ((const piece*)x)[i];
+      bytes b;
+      if (al) b = ((const bytes*)al)[i];
+#pragma unroll
+      for (int j = 0; j < E; ++j) lds[ts_pad(E * i) + j] = al && !b.v[j] ? -INFINITY : D::get(p.v[j]);
+    }
+    for (int i = whole * E + lane; i < total; i += 64) lds[ts_pad(i)] = al && !al[i] ? -INFINITY : D::get(x[i]);
+  } else {
+    const float inv = 1.f / (float)V;
+    for (int i = lane; i < total; i += 64) {
+      const int r = (int)(((float)i + 0.5f) * inv), c = i - r * V;      // i < 4096: the quotient is exact
+      lds[ts_pad(i)] = al && !al[(long)r * V + c] ? -INFINITY : D::get(x[r * row_stride + c]);
+    }
+  }
+}
+// the columns of a list that all rows share, as bits
+__device__ __forceinline__ uint64_t ts_shared_list(const unsigned char* al, int V) {
+  const bool on = (int)threadIdx.x < V && (!al || al[threadIdx.x]);
+  return __ballot(on);
+}
+
+template <class D, bool VEC>
+__global__ void __launch_bounds__(64) k_scores_small(TsArgs a) {
+  __shared__ float lds[TS_SMALL_LDS];
+  const long row0 = (long)blockIdx.x * 64, row = row0 + threadIdx.x;
+  const int n = (int)(a.rows - row0 < 64 ? a.rows - row0 : 64), V = a.V, base = threadIdx.x * V;
+  const bool own_list = a.allowed && a.allowed_stride;
+  const uint64_t on = ts_shared_list(own_list ? nullptr : a.allowed, V);
+  const int64_t t = row < a.rows ? a.tok[row] : -1;
+  ts_stage<D, VEC>((const typename D::T*)a.x + row0 * a.row_stride, own_list ? a.allowed + row0 * V : nullptr, a.row_stride, V, n, lds);
+  __syncthreads();
+  if (row >= a.rows) return;
   const float c = a.inv_temp * TS_LOG2E;
   ts_acc v = {-INFINITY, 0.f, 0.f};
-  for (int j = tid; j < a.V; j += TS_THREADS)
-    if (!al || al[j]) {
-      const float e = D::get(x + j);
-      v = ts_join(v, ts_acc{e, e == -INFINITY ? 0.f : e != e ? NAN : 1.f, 0.f}, c);
+  for (int j = 0; j < V; ++j)
+    if ((on >> j) & 1) v.m = fmaxf(v.m, lds[ts_pad(base + j)]);
+  const float r = ts_ref(v.m);
+  for (int j = 0; j < V; ++j)
+    if ((on >> j) & 1) {
+      const float d = lds[ts_pad(base + j)] - r, e = ts_exp2(c * d);
+      v.s += e;
+      v.t = fmaf(e, ts_factor(d), v.t);
     }
-  red[tid] = v;
-  for (int w = TS_THREADS / 2; w > 0; w >>= 1) {
-    __syncthreads();
-    if (tid < w) red[tid] = ts_join(red[tid], red[tid + w], c);
-  }
-  __syncthreads();
-  v = red[0];
-  if (tid == 0) ts_finish<D>(a, row, v);
-  // the k largest, one after the other: the best element that comes after the last one taken
-  float pv = INFINITY;
-  int pi = -1;
-  for (int r = 0; r < a.k; ++r) {
+  const float ls = ts_log_sum(v);
+  ts_finish(a, row, v, ls, t, t >= 0 && t < V && ((on >> t) & 1) ? lds[ts_pad(base + (int)t)] : -INFINITY);
+  for (int i = 0; i < a.k; ++i) {            // the best that is left, and out with it
     float best = -INFINITY;
-    int at = a.V;
-    for (int j = tid; j < a.V; j += TS_THREADS)
-      if (!al || al[j]) {
-        const float e = D::get(x + j);
-        if ((e < pv || (e == pv && j > pi)) && e > best) { best = e; at = j; }
+    int at = -1;
+    for (int j = 0; j < V; ++j)
+      if ((on >> j) & 1) {
+        const float x = lds[ts_pad(base + j)];
+        if (x > best) { best = x; at = j; }
       }
-    __syncthreads();
-    bv[tid] = best;
-    bi[tid] = at;
-    for (int w = TS_THREADS / 2; w > 0; w >>= 1) {
-      __syncthreads();
-      if (tid < w && (bv[tid + w] > bv[tid] || (bv[tid + w] == bv[tid] && bi[tid + w] < bi[tid]))) {
-        bv[tid] = bv[tid + w];
-        bi[tid] = bi[tid + w];
-      }
-    }
-    __syncthreads();
-    pv = bv[0];
-    pi = bi[0];
-    if (tid == 0) {
-      const long o = row * a.k + r;
-      a.top_ids[o] = pi < a.V ? pi : -1;
-      a.top_logp[o] = pi < a.V ? (v.s != v.s ? NAN : (pv - v.m) * a.inv_temp - logf(v.s)) : -INFINITY;
-    }
-    if (pi >= a.V) pv = -INFINITY;      // nothing is left: the remaining places come out the same
+    a.top_ids[row * a.k + i] = at;
+    a.top_logp[row * a.k + i] = at < 0 ? -INFINITY : ts_logp(best, v, ls, a.inv_temp);
+    if (at >= 0) lds[ts_pad(base + at)] = -INFINITY;
   }
 }
 
@@ -147,81 +188,514 @@ struct TsBwdArgs {
   const void* x;
   const int64_t* tok;
   const unsigned char* allowed;
-  long allowed_stride, row_stride;
-  const float *stats, *entropy, *g_logp, *g_entropy, *g_top;
+  long allowed_stride, row_stride, rows;
+  const float *stats, *logp, *entropy, *g_logp, *g_entropy, *g_top;
   const int64_t* top_ids;
   void* dx;
-  int V, k;
+  int V, k, splits, per_part;
   float inv_temp;
 };
 
-template <class D>
-__global__ void __launch_bounds__(TS_THREADS) k_token_scores_bwd(TsBwdArgs a) {
-  const long row = blockIdx.x;
-  const typename D::T* x = (const typename D::T*)a.x + row * a.row_stride;
-  typename D::T* dx = (typename D::T*)a.dx + row * a.V;
-  const unsigned char* al = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
-  const float m = a.stats[2 * row], ls = a.stats[2 * row + 1];
-  const float gh = a.g_entropy ? a.g_entropy[row] : 0.f, H = a.g_entropy ? a.entropy[row] : 0.f;
-  const int64_t t = a.tok[row];
-  float g1 = 0.f;
-  if (a.g_logp && t >= 0 && t < a.V && (!al || al[t]) && D::get(x + t) != -INFINITY) g1 = a.g_logp[row];
-  float whole = g1;
+// What a row's gradient is made of: d_j = inv_temp * (hot_j - p_j * (whole + gh * (logp_j + H)))
+struct TsRowGrad {
+  float m, ls, gh, H, g1, whole;
+  int64_t t;
+};
+__device__ __forceinline__ TsRowGrad ts_row_grad(const TsBwdArgs& a, long row) {
+  TsRowGrad g;
+  const float2 st = *(const float2*)(a.stats + 2 * row);
+  g.m = st.x;
+  g.ls = st.y;
+  g.gh = a.g_entropy ? a.g_entropy[row] : 0.f;
+  g.H = a.g_entropy ? a.entropy[row] : 0.f;
+  g.t = a.tok[row];
+  g.g1 = a.g_logp && g.t >= 0 && g.t < a.V && a.logp[row] != -INFINITY ? a.g_logp[row] : 0.f;
+  g.whole = g.g1;
   for (int r = 0; r < a.k; ++r)
-    if (a.top_ids[row * a.k + r] >= 0) whole += a.g_top[row * a.k + r];
-  __syncthreads();                      // dlogits may be the logits: x_t has been read by every thread
-  for (int j = threadIdx.x; j < a.V; j += TS_THREADS) {
-    const float e = D::get(x + j);
-    float d = 0.f;
-    if ((!al || al[j]) && e != -INFINITY) {
-      const float lp = (e - m) * a.inv_temp - ls, p = ts_exp2(lp * TS_LOG2E);
-      d = -p * (whole + gh * (ts_factor(lp) + H));
-      if (j == t) d += g1;
-      for (int r = 0; r < a.k; ++r)
-        if (a.top_ids[row * a.k + r] == j) d += a.g_top[row * a.k + r];
-      d *= a.inv_temp;
+    if (a.top_ids[row * a.k + r] >= 0) g.whole += a.g_top[row * a.k + r];
+  return g;
+}
+__device__ __forceinline__ float ts_dense_grad(float x, const TsRowGrad& g, float inv_temp) {
+  const float lp = (x - g.m) * inv_temp - g.ls, p = ts_exp2(lp * TS_LOG2E);
+  return x == -INFINITY ? 0.f : -p * (g.whole + g.gh * (ts_factor(lp) + g.H));
+}
+// what the one-hot terms add to column j
+__device__ __forceinline__ float ts_hot(const TsBwdArgs& a, long row, const TsRowGrad& g, int64_t j) {
+  float h = j == g.t ? g.g1 : 0.f;
+  for (int r = 0; r < a.k; ++r)
+    if (a.top_ids[row * a.k + r] == j) h += a.g_top[row * a.k + r];
+  return h;
+}
+
+template <class D, bool VEC>
+__global__ void __launch_bounds__(64) k_scores_small_bwd(TsBwdArgs a) {
+  constexpr int E = 16 / sizeof(typename D::T);
+  __shared__ float lds[TS_SMALL_LDS];
+  const long row0 = (long)blockIdx.x * 64, row = row0 + threadIdx.x;
+  const int n = (int)(a.rows - row0 < 64 ? a.rows - row0 : 64), V = a.V, base = threadIdx.x * V;
+  const bool own_list = a.allowed && a.allowed_stride;
+  const uint64_t on = ts_shared_list(own_list ? nullptr : a.allowed, V);
+  ts_stage<D, VEC>((const typename D::T*)a.x + row0 * a.row_stride, own_list ? a.allowed + row0 * V : nullptr, a.row_stride, V, n, lds);
+  __syncthreads();
+  if (row < a.rows) {
+    const TsRowGrad g = ts_row_grad(a, row);
+    for (int j = 0; j < V; ++j) {
+      float* p = lds + ts_pad(base + j);
+      *p = (on >> j) & 1 ? ts_dense_grad(*p, g, a.inv_temp) * a.inv_temp : 0.f;
     }
-    dx[j] = D::put(d);
+    if (g.g1 != 0.f) lds[ts_pad(base + (int)g.t)] += g.g1 * a.inv_temp;
+    for (int r = 0; r < a.k; ++r) {
+      const int64_t j = a.top_ids[row * a.k + r];
+      if (j >= 0 && j < V) lds[ts_pad(base + (int)j)] += a.g_top[row * a.k + r] * a.inv_temp;
+    }
   }
+  __syncthreads();
+  typename D::T* dx = (typename D::T*)a.dx + row0 * V;
+  const int total = n * V, whole = VEC ? total / E : 0;
+  for (int i = threadIdx.x; i < whole; i += 64) {
+    struct alignas(16) piece { typename D::T v[E]; } p;
+#pragma unroll
+    for (int j = 0; j < E; ++j) p.v[j] = D::put(lds[ts_pad(E * i) + j]);
+    ((piece*)dx)[i] = p;
+  }
+  for (int i = whole * E + threadIdx.x; i < total; i += 64) dx[i] = D::put(lds[ts_pad(i)]);
+}
+
+// ---------------------------------------------------------------------------------------------- longer rows
+// A row as 16-byte pieces: piece c holds elements [c * E - skew, c * E - skew + E), skew = the row's distance from the
+// 16-byte boundary before it.  The first and the last piece may stick out of the row: they are read element by element.
+template <class D>
+struct TsRow {
+  static constexpr int E = 16 / sizeof(typename D::T);
+  struct alignas(16) piece { typename D::T v[E]; };
+  const typename D::T* x;
+  const unsigned char* al;
+  int V, skew, pieces;
+  __device__ __forceinline__ TsRow(const void* base, const unsigned char* allowed, long row, long row_stride, long allowed_stride, int V_) {
+    x = (const typename D::T*)base + row * row_stride;
+    al = allowed ? allowed + row * allowed_stride : nullptr;
+    V = V_;
+    skew = (int)(((uintptr_t)x & 15) / sizeof(typename D::T));
+    pieces = (int)(((long)V + skew + E - 1) / E);
+  }
+  __device__ __forceinline__ bool inside(int c) const { return (c > 0 || skew == 0) && (long)c * E - skew + E <= V; }
+  // the elements of piece c as floats, -inf where no column counts
+  __device__ __forceinline__ void load(int c, float v[E]) const {
+    const int j0 = c * E - skew;
+    if (inside(c)) {
+      const piece p = *(const piece*)(x + j0);
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[j] = D::get(p.v[j]);
+      if (al) {
+        unsigned char b[E];
+        __builtin_memcpy(b, al + j0, E);
+#pragma unroll
+        for (int j = 0; j < E; ++j) v[j] = b[j] ? v[j] : -INFINITY;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[j] = j0 + j >= 0 && j0 + j < V && (!al || al[j0 + j]) ? D::get(x[j0 + j]) : -INFINITY;
+    }
+  }
+};
+
+// floats as unsigned integers of the same order (no NaN among them)
+__device__ __forceinline__ unsigned ts_key(float v) {
+  const unsigned u = __float_as_uint(v + 0.f);            // -0 -> 0: the two are equal
+  return u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float ts_unkey(unsigned k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
+
+#define TS_LIST 512
+struct TsList {
+  int n;
+  float x[TS_LIST];
+  int at[TS_LIST];
+};
+__device__ __forceinline__ bool ts_before(float x, int at, float y, int bt) { return x > y || (x == y && at < bt); }
+
+// The k best of the elements of pieces [c0, c1), which this workgroup's threads walked in steps of T with maxima `mine`.
+// put(i, x, at) receives the i-th best; n, the number found, is returned to every thread.
+template <class D, int T, class Put>
+__device__ __forceinline__ int ts_top(const TsRow<D>& R, int c0, int c1, float mine, int k, TsList* list, unsigned* wave_bound, Put put) {
+  constexpr int E = TsRow<D>::E;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  // the k-th largest of the wave's maxima, rounded down to 16 bits
+  const unsigned key = ts_key(mine);
+  unsigned bound = 0;
+#pragma unroll
+  for (int b = 31; b >= 16; --b) {
+    const unsigned c = bound | (1u << b);
+    if (__popcll(__ballot(key >= c)) >= k) bound = c;
+  }
+  if (tid == 0) list->n = 0;
+  if (lane == 0) wave_bound[wave] = bound;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < T / 64; ++w) bound = wave_bound[w] > bound ? wave_bound[w] : bound;
+  const float least = bound < 0x00800000u ? -INFINITY : ts_unkey(bound);     // (smaller keys are -inf's own, rounded down)
+  for (uint64_t todo = __ballot(key >= bound && mine > -INFINITY); todo; todo &= todo - 1) {
+    const int first = c0 + wave * 64 + (int)__builtin_ctzll(todo);      // the wave reads that thread's pieces together
+    for (long c = first + (long)T * lane; c < c1; c += (long)T * 64) {
+      float v[E];
+      R.load((int)c, v);
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (v[j] > -INFINITY && v[j] >= least) {
+          const int p = atomicAdd(&list->n, 1);
+          if (p < TS_LIST) {
+            list->x[p] = v[j];
+            list->at[p] = (int)c * E - R.skew + j;
+          }
+        }
+    }
+  }
+  __syncthreads();
+  const int n = list->n;
+  if (n <= TS_LIST) {                        // the order of the list does not matter: every entry finds its own place
+    for (int i = tid; i < n; i += T) {
+      const float x = list->x[i];
+      const int at = list->at[i];
+      int place = 0;
+      for (int o = 0; o < n; ++o) place += ts_before(list->x[o], list->at[o], x, at);
+      if (place < k) put(place, x, at);
+    }
+    return n < k ? n : k;
+  }
+  float px = INFINITY;
+  int pat = -1, found = 0;
+  for (; found < k; ++found) {               // too many equals: one search per place
+    float best = -INFINITY;
+    int at = 0x7fffffff;
+    for (int c = c0 + tid; c < c1; c += T) {
+      float v[E];
+      R.load(c, v);
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const int i = c * E - R.skew + j;
+        if (v[j] > -INFINITY && ts_before(px, pat, v[j], i) && ts_before(v[j], i, best, at)) { best = v[j]; at = i; }
+      }
+    }
+#pragma unroll
+    for (int w = 32; w > 0; w >>= 1) {
+      const float ox = __shfl_xor(best, w);
+      const int oi = __shfl_xor(at, w);
+      if (ts_before(ox, oi, best, at)) { best = ox; at = oi; }
+    }
+    __syncthreads();
+    if (lane == 0) { list->x[wave] = best; list->at[wave] = at; }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < T / 64; ++w)
+      if (ts_before(list->x[w], list->at[w], best, at)) { best = list->x[w]; at = list->at[w]; }
+    if (best == -INFINITY) break;            // (uniform)
+    if (tid == 0) put(found, best, at);
+    px = best;
+    pat = at;
+  }
+  return found;
+}
+
+#define TS_BATCH 4              // pieces that a thread requests before it uses the first
+
+template <class D, int T>
+__global__ void __launch_bounds__(T) k_scores_row(TsArgs a) {
+  constexpr int E = TsRow<D>::E;
+  __shared__ TsList list;
+  __shared__ ts_acc wave_acc[T / 64];
+  __shared__ unsigned wave_bound[T / 64];
+  const int tid = threadIdx.x;
+  const long row = a.splits == 1 ? blockIdx.x : blockIdx.x / a.splits;
+  const int part = a.splits == 1 ? 0 : (int)(blockIdx.x % a.splits);
+  const TsRow<D> R(a.x, a.allowed, row, a.row_stride, a.allowed_stride, a.V);
+  const int c0 = part * a.per_part, c1 = part == a.splits - 1 || c0 + a.per_part > R.pieces ? R.pieces : c0 + a.per_part;
+  const float c = a.inv_temp * TS_LOG2E;
+  int64_t t = -1;
+  float xt = -INFINITY;
+  if (tid == 0 && a.splits == 1) {           // requested ahead of the row
+    t = a.tok[row];
+    xt = ts_token<D>(a, row, t);
+  }
+  ts_acc v = {-INFINITY, 0.f, 0.f};
+  for (long i = c0 + tid; i < c1; i += (long)T * TS_BATCH) {
+    float x[TS_BATCH][E];
+#pragma unroll
+    for (int u = 0; u < TS_BATCH; ++u) {
+      if (i + (long)T * u < c1) {
+        R.load((int)(i + T * u), x[u]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j) x[u][j] = -INFINITY;
+      }
+    }
+    float m = v.m;
+#pragma unroll
+    for (int u = 0; u < TS_BATCH; ++u)
+#pragma unroll
+      for (int j = 0; j < E; ++j) m = fmaxf(m, x[u][j]);
+    const float r = ts_ref(m);
+    if (m > v.m) {                           // the running sums move to the new maximum
+      const float d = v.m - r, f = ts_exp2(c * d);
+      v.t = (v.t + v.s * ts_factor(d)) * f;
+      v.s *= f;
+      v.m = m;
+    }
+#pragma unroll
+    for (int u = 0; u < TS_BATCH; ++u)
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const float d = x[u][j] - r, e = ts_exp2(c * d);
+        v.s += e;
+        v.t = fmaf(e, ts_factor(d), v.t);
+      }
+  }
+  const float mine = v.m;
+  v = ts_join_wave(v, c);
+  if (T > 64) {
+    if ((tid & 63) == 0) wave_acc[tid >> 6] = v;
+    __syncthreads();
+    v = wave_acc[0];
+#pragma unroll
+    for (int w = 1; w < T / 64; ++w) v = ts_join(v, wave_acc[w], c);
+  }
+  const float ls = ts_log_sum(v);
+  if (a.splits > 1) {
+    TsPart* P = (TsPart*)a.parts + row * a.splits + part;
+    int n = 0;
+    if (a.k) n = ts_top<D, T>(R, c0, c1, mine, a.k, &list, wave_bound, [&](int i, float x, int at) {
+      P->x[i] = x;
+      P->at[i] = at;
+    });
+    if (tid == 0) {
+      P->v = v;
+      P->n = n;
+    }
+    return;
+  }
+  if (tid == 0) ts_finish(a, row, v, ls, t, xt);
+  if (a.k == 0) return;
+  const int n = ts_top<D, T>(R, c0, c1, mine, a.k, &list, wave_bound, [&](int i, float x, int at) {
+    a.top_ids[row * a.k + i] = at;
+    a.top_logp[row * a.k + i] = ts_logp(x, v, ls, a.inv_temp);
+  });
+  for (int i = n + tid; i < a.k; i += T) {
+    a.top_ids[row * a.k + i] = -1;
+    a.top_logp[row * a.k + i] = -INFINITY;
+  }
+}
+
+#define TS_MAX_SPLITS 64
+// The parts of a row, joined: the sums in the order of the parts (every thread the same), the alternatives by counting
+// for each of the parts' own k best how many of the others come before it.
+template <class D>
+__global__ void __launch_bounds__(256) k_scores_join(TsArgs a) {
+  __shared__ float lx[TS_MAX_SPLITS * DRK_TOPK_MAX];
+  __shared__ int lat[TS_MAX_SPLITS * DRK_TOPK_MAX];
+  __shared__ ts_acc lv[TS_MAX_SPLITS];
+  __shared__ int found;
+  const long row = blockIdx.x;
+  const int tid = threadIdx.x;
+  const TsPart* P = (const TsPart*)a.parts + row * a.splits;
+  const float c = a.inv_temp * TS_LOG2E;
+  const int total = a.splits * a.k;
+  if (tid == 0) found = 0;
+  __syncthreads();
+  if (tid < a.splits) {
+    lv[tid] = P[tid].v;
+    if (a.k) atomicAdd(&found, P[tid].n);
+  }
+  for (int i = tid; i < total; i += 256) {
+    const int p = i / a.k, j = i % a.k;
+    const bool on = j < P[p].n;
+    lx[i] = on ? P[p].x[j] : -INFINITY;
+    lat[i] = on ? P[p].at[j] : 0x7fffffff;
+  }
+  __syncthreads();
+  ts_acc v = lv[0];
+  for (int p = 1; p < a.splits; ++p) v = ts_join(v, lv[p], c);
+  const float ls = ts_log_sum(v);
+  if (tid == 0) {
+    const int64_t t = a.tok[row];
+    ts_finish(a, row, v, ls, t, ts_token<D>(a, row, t));
+  }
+  for (int i = tid; i < total; i += 256) {
+    const float x = lx[i];
+    const int at = lat[i];
+    if (x == -INFINITY) continue;
+    int place = 0;
+    for (int o = 0; o < total; ++o) place += ts_before(lx[o], lat[o], x, at);
+    if (place < a.k) {
+      a.top_ids[row * a.k + place] = at;
+      a.top_logp[row * a.k + place] = ts_logp(x, v, ls, a.inv_temp);
+    }
+  }
+  for (int i = found + tid; i < a.k; i += 256) {
+    a.top_ids[row * a.k + i] = -1;
+    a.top_logp[row * a.k + i] = -INFINITY;
+  }
+}
+
+// One pass: piece in, piece out.  The columns of the one-hot terms are stored once more at the end, by a thread each, from
+// logits that were read before the first store (dlogits may be the logits: a workgroup reads only what it writes itself).
+// ALIKE: a row of dlogits lies on the 16-byte grid as the row of logits does, so that whole pieces are stored.
+template <class D, int T, bool ALIKE>
+__global__ void __launch_bounds__(T) k_scores_row_bwd(TsBwdArgs a) {
+  constexpr int E = TsRow<D>::E;
+  const int tid = threadIdx.x;
+  const long row = a.splits == 1 ? blockIdx.x : blockIdx.x / a.splits;
+  const int part = a.splits == 1 ? 0 : (int)(blockIdx.x % a.splits);
+  const TsRow<D> R(a.x, a.allowed, row, a.row_stride, a.allowed_stride, a.V);
+  const int c0 = part * a.per_part, c1 = part == a.splits - 1 || c0 + a.per_part > R.pieces ? R.pieces : c0 + a.per_part;
+  typename D::T* dx = (typename D::T*)a.dx + row * a.V;
+  const TsRowGrad g = ts_row_grad(a, row);
+  int64_t mine = -1;
+  float xm = -INFINITY;
+  if (tid <= a.k) {
+    mine = tid < a.k ? a.top_ids[row * a.k + tid] : g.g1 != 0.f ? g.t : -1;
+    const long piece = mine < 0 || mine >= a.V ? -1 : (mine + R.skew) / E;
+    if (piece >= c0 && piece < c1) xm = D::get(R.x[mine]);
+    else mine = -1;
+  }
+  if (T > 64) __syncthreads();
+  for (long i = c0 + tid; i < c1; i += (long)T * TS_BATCH) {
+    float x[TS_BATCH][E];
+#pragma unroll
+    for (int u = 0; u < TS_BATCH; ++u)
+      if (i + (long)T * u < c1) R.load((int)(i + T * u), x[u]);
+#pragma unroll
+    for (int u = 0; u < TS_BATCH; ++u) {
+      if (i + (long)T * u >= c1) continue;
+      const int c = (int)(i + T * u), j0 = c * E - R.skew;
+      typename TsRow<D>::piece p;
+#pragma unroll
+      for (int j = 0; j < E; ++j) p.v[j] = D::put(ts_dense_grad(x[u][j], g, a.inv_temp) * a.inv_temp);
+      if (ALIKE && R.inside(c)) {
+        *(typename TsRow<D>::piece*)(dx + j0) = p;
+      } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          if (j0 + j >= 0 && j0 + j < a.V) dx[j0 + j] = p.v[j];
+      }
+    }
+  }
+  __syncthreads();
+  if (mine >= 0) dx[mine] = D::put((ts_dense_grad(xm, g, a.inv_temp) + ts_hot(a, row, g, mine)) * a.inv_temp);
 }
 
 // ------------------------------------------------------------------------------------------------ C ABI
 static bool ts_shape_ok(long rows, int V, long row_stride, long allowed_stride, int k, float temp) {
-  return rows >= 0 && rows < (1L << 31) && V >= 1 && row_stride >= 0 && (allowed_stride == 0 || allowed_stride >= V) && k >= 0 &&
-         k <= DRK_TOPK_MAX && k <= V && temp > 0.f && temp < INFINITY && 1.f / temp < INFINITY;
+  return rows >= 0 && rows < (1L << 31) && V >= 1 && V <= (1 << 30) && row_stride >= 0 && (allowed_stride == 0 || allowed_stride >= V) &&
+         k >= 0 && k <= DRK_TOPK_MAX && k <= V && temp > 0.f && temp < INFINITY && 1.f / temp < INFINITY;
+}
+static int ts_size(int dtype) { return dtype == DRK_F32 ? 4 : 2; }
+
+// Pieces of 16 bytes per row (one more when the row may start inside one), threads per row, parts per row.  A row of up to
+// 256 pieces is one wave's: its four loads per lane are in flight together.  With fewer rows than `want` workgroups, a row
+// is split as long as a part keeps one piece per thread.
+static void ts_plan(long rows, int V, int size, long want, bool* wave, int* splits, int* per_part) {
+  const int e = 16 / size;
+  const long pieces = ((long)V + e - 1) / e + 1;
+  *wave = pieces <= 256;
+  long s = 1;
+  if (!*wave && rows < want) {
+    s = (want + rows - 1) / rows;
+    if (s > pieces / 256) s = pieces / 256;
+    if (s > TS_MAX_SPLITS) s = TS_MAX_SPLITS;
+    if (s < 1) s = 1;
+  }
+  const long per = (pieces + s - 1) / s;
+  *per_part = (int)per;
+  *splits = (int)((pieces + per - 1) / per);
+}
+#define TS_WANT_FWD 512
+
+extern "C" long drk_token_scores_workspace_bytes(long rows, int V, int dtype) {
+  if (rows <= 0 || V <= TS_SMALL_V) return 0;
+  bool wave;
+  int splits, per;
+  ts_plan(rows, V, ts_size(dtype), TS_WANT_FWD, &wave, &splits, &per);
+  return splits == 1 ? 0 : rows * splits * (long)sizeof(TsPart);
+}
+
+template <class D>
+static int ts_forward(TsArgs a, bool dense, hipStream_t st) {
+  if (a.V <= TS_SMALL_V) {
+    const bool vec = dense && ((uintptr_t)a.x & 15) == 0 && (!a.allowed_stride || ((uintptr_t)a.allowed & 7) == 0);
+    const dim3 grid((unsigned)((a.rows + 63) / 64));
+    if (vec) hipLaunchKernelGGL((k_scores_small<D, true>), grid, dim3(64), 0, st, a);
+    else hipLaunchKernelGGL((k_scores_small<D, false>), grid, dim3(64), 0, st, a);
+    DRK_CHECK_LAUNCH();
+    return DRK_OK;
+  }
+  bool wave;
+  ts_plan(a.rows, a.V, (int)sizeof(typename D::T), TS_WANT_FWD, &wave, &a.splits, &a.per_part);
+  const dim3 grid((unsigned)(a.rows * a.splits));
+  if (wave) hipLaunchKernelGGL((k_scores_row<D, 64>), grid, dim3(64), 0, st, a);
+  else hipLaunchKernelGGL((k_scores_row<D, 256>), grid, dim3(256), 0, st, a);
+  DRK_CHECK_LAUNCH();
+  if (a.splits > 1) {
+    hipLaunchKernelGGL(k_scores_join<D>, dim3((unsigned)a.rows), dim3(256), 0, st, a);
+    DRK_CHECK_LAUNCH();
+  }
+  return DRK_OK;
 }
 
 extern "C" int drk_token_scores(const void* logits, int dtype, long row_stride, const int64_t* tokens, const unsigned char* allowed,
                                 long allowed_stride, float temp, int k, float* logp, float* entropy, int64_t* top_ids,
-                                float* top_logp, float* stats, long rows, int V, void* stream) {
+                                float* top_logp, float* stats, long rows, int V, void* workspace, long workspace_bytes, void* stream) {
   TSCHECK(ts_shape_ok(rows, V, row_stride, allowed_stride, k, temp), "drk_token_scores (rows, V, strides, k or temp)");
   if (rows == 0) return DRK_OK;
   TSCHECK(logits && tokens && logp && stats && (k == 0 || (top_ids && top_logp)), "drk_token_scores");
-  const TsArgs a = {logits, tokens, allowed, allowed_stride, row_stride, logp, entropy, stats, top_logp, top_ids, V, k, 1.f / temp};
-  const dim3 grid((unsigned)rows), block(TS_THREADS);
-  hipStream_t st = (hipStream_t)stream;
-  if (dtype == DRK_F32) hipLaunchKernelGGL(k_token_scores<ts_f32>, grid, block, 0, st, a);
-  else if (dtype == DRK_BF16) hipLaunchKernelGGL(k_token_scores<ts_bf16>, grid, block, 0, st, a);
-  else if (dtype == DRK_F16) hipLaunchKernelGGL(k_token_scores<ts_f16>, grid, block, 0, st, a);
-  else return drk_set_error_msg(DRK_EINVAL, "drk_token_scores: dtype is DRK_F32, DRK_BF16 or DRK_F16");
+  TSCHECK(((uintptr_t)stats & 7) == 0, "drk_token_scores (stats: 8-byte aligned)");
+  const long need = drk_token_scores_workspace_bytes(rows, V, dtype);
+  TSCHECK(need == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need),
+          "drk_token_scores (workspace: 16-byte aligned, drk_token_scores_workspace_bytes(rows, V, dtype) bytes)");
+  const TsArgs a = {logits, tokens, allowed, allowed_stride, row_stride, rows, logp, entropy, stats, top_logp, top_ids, workspace, V, k, 1, 0, 1.f / temp};
+  const bool dense = row_stride == V && (allowed_stride == 0 || allowed_stride == V);
+  if (dtype == DRK_F32) return ts_forward<ts_f32>(a, dense, (hipStream_t)stream);
+  if (dtype == DRK_BF16) return ts_forward<ts_bf16>(a, dense, (hipStream_t)stream);
+  if (dtype == DRK_F16) return ts_forward<ts_f16>(a, dense, (hipStream_t)stream);
+  return drk_set_error_msg(DRK_EINVAL, "drk_token_scores: dtype is DRK_F32, DRK_BF16 or DRK_F16");
+}
+
+#define TS_WANT_BWD 1024
+template <class D>
+static int ts_backward(TsBwdArgs a, bool dense, hipStream_t st) {
+  const int size = (int)sizeof(typename D::T);
+  if (a.V <= TS_SMALL_V) {
+    const bool vec = dense && ((uintptr_t)a.x & 15) == 0 && ((uintptr_t)a.dx & 15) == 0 && (!a.allowed_stride || ((uintptr_t)a.allowed & 7) == 0);
+    const dim3 grid((unsigned)((a.rows + 63) / 64));
+    if (vec) hipLaunchKernelGGL((k_scores_small_bwd<D, true>), grid, dim3(64), 0, st, a);
+    else hipLaunchKernelGGL((k_scores_small_bwd<D, false>), grid, dim3(64), 0, st, a);
+    DRK_CHECK_LAUNCH();
+    return DRK_OK;
+  }
+  bool wave;
+  ts_plan(a.rows, a.V, size, TS_WANT_BWD, &wave, &a.splits, &a.per_part);
+  const bool alike = (a.row_stride - a.V) * size % 16 == 0 && (((uintptr_t)a.x ^ (uintptr_t)a.dx) & 15) == 0;
+  const dim3 grid((unsigned)(a.rows * a.splits));
+  if (wave && alike) hipLaunchKernelGGL((k_scores_row_bwd<D, 64, true>), grid, dim3(64), 0, st, a);
+  else if (wave) hipLaunchKernelGGL((k_scores_row_bwd<D, 64, false>), grid, dim3(64), 0, st, a);
+  else if (alike) hipLaunchKernelGGL((k_scores_row_bwd<D, 256, true>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((k_scores_row_bwd<D, 256, false>), grid, dim3(256), 0, st, a);
   DRK_CHECK_LAUNCH();
   return DRK_OK;
 }
 
 extern "C" int drk_token_scores_bwd(const void* logits, int dtype, long row_stride, const int64_t* tokens,
                                     const unsigned char* allowed, long allowed_stride, float temp, int k, const float* stats,
-                                    const float* entropy, const int64_t* top_ids, const float* g_logp, const float* g_entropy,
-                                    const float* g_top, void* dlogits, long rows, int V, void* stream) {
+                                    const float* logp, const float* entropy, const int64_t* top_ids, const float* g_logp,
+                                    const float* g_entropy, const float* g_top, void* dlogits, long rows, int V, void* stream) {
   TSCHECK(ts_shape_ok(rows, V, row_stride, allowed_stride, k, temp), "drk_token_scores_bwd (rows, V, strides, k or temp)");
   if (rows == 0) return DRK_OK;
-  TSCHECK(logits && tokens && stats && dlogits && (!g_entropy || entropy) && (k == 0 || (top_ids && g_top)), "drk_token_scores_bwd");
-  const TsBwdArgs a = {logits, tokens, allowed, allowed_stride, row_stride, stats, entropy, g_logp, g_entropy, g_top, top_ids, dlogits, V, k, 1.f / temp};
-  const dim3 grid((unsigned)rows), block(TS_THREADS);
-  hipStream_t st = (hipStream_t)stream;
-  if (dtype == DRK_F32) hipLaunchKernelGGL(k_token_scores_bwd<ts_f32>, grid, block, 0, st, a);
-  else if (dtype == DRK_BF16) hipLaunchKernelGGL(k_token_scores_bwd<ts_bf16>, grid, block, 0, st, a);
-  else if (dtype == DRK_F16) hipLaunchKernelGGL(k_token_scores_bwd<ts_f16>, grid, block, 0, st, a);
-  else return drk_set_error_msg(DRK_EINVAL, "drk_token_scores_bwd: dtype is DRK_F32, DRK_BF16 or DRK_F16");
-  DRK_CHECK_LAUNCH();
-  return DRK_OK;
+  TSCHECK(logits && tokens && stats && dlogits && (!g_logp || logp) && (!g_entropy || entropy) && (k == 0 || (top_ids && g_top)),
+          "drk_token_scores_bwd");
+  TSCHECK(((uintptr_t)stats & 7) == 0, "drk_token_scores_bwd (stats: 8-byte aligned)");
+  TSCHECK(dlogits != logits || row_stride == V, "drk_token_scores_bwd (in place: dense rows)");
+  const TsBwdArgs a = {logits, tokens, allowed, allowed_stride, row_stride, rows, stats, logp, entropy, g_logp, g_entropy, g_top, top_ids, dlogits, V, k, 1, 0, 1.f / temp};
+  const bool dense = row_stride == V && (allowed_stride == 0 || allowed_stride == V);
+  if (dtype == DRK_F32) return ts_backward<ts_f32>(a, dense, (hipStream_t)stream);
+  if (dtype == DRK_BF16) return ts_backward<ts_bf16>(a, dense, (hipStream_t)stream);
+  if (dtype == DRK_F16) return ts_backward<ts_f16>(a, dense, (hipStream_t)stream);
+  return drk_set_error_msg(DRK_EINVAL, "drk_token_scores_bwd: dtype is DRK_F32, DRK_BF16 or DRK_F16");
 }

@@ -679,8 +679,10 @@ def token_scores(logits, tokens, *, allowed=None, temp=1.0, topk=0, entropy=True
     new = lambda *last, dtype=torch.float32: torch.empty(*tokens.shape, *last, dtype=dtype, device=logits.device)
     s = TokenScores(new(), new() if entropy else None, new(topk, dtype=torch.int64) if topk else None,
                     new(topk) if topk else None, new(2))
+    need = _lib.load().drk_token_scores_workspace_bytes(tokens.numel(), V, args[1])
+    ws = _scratch(need, logits.device) if need else None
     _lib.call('drk_token_scores', *args, topk, _raw(s.logp), _raw(s.entropy), _raw(s.top_ids), _raw(s.top_logp), _raw(s.stats),
-              tokens.numel(), V, _stream())
+              tokens.numel(), V, _raw(ws), need, _stream())
     return s
 
 
@@ -696,12 +698,12 @@ def token_scores_bwd(logits, tokens, scores, *, g_logp=None, g_entropy=None, g_t
         raise ValueError('token_scores_bwd: g_top needs the top alternatives')
     k = scores.top_ids.shape[-1] if g_top is not None else 0
     for t, want, name in ((g_logp, shape, 'g_logp'), (g_entropy, shape, 'g_entropy'), (g_top, shape + (k,), 'g_top'),
-                          (scores.stats, shape + (2,), 'stats'), (out, tuple(logits.shape), 'out')):
+                          (scores.stats, shape + (2,), 'stats'), (scores.logp, shape, 'logp'), (out, tuple(logits.shape), 'out')):
         if t is not None and tuple(t.shape) != want:
             raise ValueError(f'token_scores_bwd: {name} has shape {want}, got {tuple(t.shape)}')
     out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if out is None else out
-    _here('token_scores_bwd', g_logp, g_entropy, g_top, scores.stats, out)
-    _lib.call('drk_token_scores_bwd', *args, k, _f(scores.stats, 'stats'), _f(scores.entropy, 'entropy') if g_entropy is not None else None,
+    _here('token_scores_bwd', g_logp, g_entropy, g_top, *scores, out)
+    _lib.call('drk_token_scores_bwd', *args, k, _f(scores.stats, 'stats'), _f(scores.logp, 'logp'), _f(scores.entropy, 'entropy') if g_entropy is not None else None,
               _i(scores.top_ids, 'top_ids') if k else None, _f(g_logp, 'g_logp'), _f(g_entropy, 'g_entropy'), _f(g_top, 'g_top'),
               _dev_ptr(out, logits.dtype, 'out'), tokens.numel(), V, _stream())
     return out

@@ -128,13 +128,15 @@ int drk_likelihood_accum(const float* logits, const int64_t* x0, const int64_t* 
 #define DRK_TOPK_MAX 32
 int drk_token_scores(const void* logits, int dtype, long row_stride, const int64_t* tokens, const unsigned char* allowed,
                      long allowed_stride, float temp, int k, float* logp, float* entropy, int64_t* top_ids,
-                     float* top_logp, float* stats, long rows, int V, void* stream);
+                     float* top_logp, float* stats, long rows, int V, void* workspace, long workspace_bytes, void* stream);
+/* Few long rows are split over workgroups: bytes of the 16-byte aligned workspace for their partial results (0: none). */
+long drk_token_scores_workspace_bytes(long rows, int V, int dtype);
 /* Gradient of sum g_logp logp + sum g_entropy entropy + sum g_top top_logp with respect to the logits (each g optional;
- * g_entropy needs the entropy, g_top the ids that the forward gave, else k = 0).  dlogits [rows][V], dense, of the logits'
+ * g_logp needs the logp, g_entropy the entropy, g_top the ids that the forward gave, else k = 0).  dlogits [rows][V], dense, of the logits'
  * type, every element written: 0 in columns that do not count; it may be the logits themselves when they are dense.  A log-probability of -inf, 0 (not scored) or NaN (token
  * >= V) passes no gradient, nor does a place with id -1. */
 int drk_token_scores_bwd(const void* logits, int dtype, long row_stride, const int64_t* tokens, const unsigned char* allowed,
-                         long allowed_stride, float temp, int k, const float* stats, const float* entropy,
+                         long allowed_stride, float temp, int k, const float* stats, const float* logp, const float* entropy,
                          const int64_t* top_ids, const float* g_logp, const float* g_entropy, const float* g_top,
                          void* dlogits, long rows, int V, void* stream);
 

@@ -254,7 +254,7 @@ def test_refusals_cpu():
     def rc(**kw):
         a = {**ok, **kw}
         return lib.drk_token_scores(None, a['dtype'], a['stride'], None, None, a['ast'], a['temp'], a['k'], None, None, None, None,
-                                    None, a['rows'], a['V'], None)
+                                    None, a['rows'], a['V'], None, 0, None)
     assert rc(rows=0) == 0                              # an empty batch is a no-op, whatever its pointers
     for bad in (dict(), dict(V=0), dict(rows=-1), dict(temp=0.0), dict(temp=-1.0), dict(temp=math.inf), dict(temp=math.nan),
                 dict(temp=1e-45), dict(k=6), dict(k=-1), dict(k=33, V=100), dict(ast=3), dict(stride=-1)):
