@@ -85,7 +85,7 @@ HOST_QUERIES = {
     'drk_gate_bf16_workspace_bytes': [],
     'drk_token_scores_workspace_bytes': [c_long, c_int, c_int],
     'drk_ln_bwd_ck8_workspace_bytes': [c_int, c_int],
-    'drk_conv_wgrad_ck8_workspace_bytes': [c_int, c_int, c_int],
+    'drk_conv_wgrad_ck8_workspace_bytes': [c_int, c_int, c_int, c_int],
     'drk_conv_wgrad_bf16_multi_workspace_bytes': [c_int, c_int, c_int, c_int],
     'drk_head_bwd_bf16_slab_floats': [],
     'drk_denoiser_bwd_bf16_slab_floats': [c_int],

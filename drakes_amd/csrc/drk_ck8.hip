@@ -12,6 +12,8 @@
 //   weight gradient:     h = gamma * xq + beta, so  dw[t] = gamma (x) P[t] + beta (x) S[t],
 //                        P[t][ci][co] = sum_rows xq[row + off_t][ci] dc[row][co],  S[t][co] = sum of dc over the rows that
 //                        tap t can reach: gamma and beta stay out of the matrix product, where h would have to be rounded.
+#include <atomic>
+
 #include "drk_common.h"
 #include "../../include/drakes_hip.h"
 
@@ -278,108 +280,427 @@ __global__ void __launch_bounds__(256) k_ck8_sums(const float* __restrict__ slab
 }
 
 // ---- weight gradient -----------------------------------------------------------------------------------------------
-// Workgroup = (chunk of rows, tap).  Tiles of 64 rows of xq (decoded to bf16, shifted by the tap) and of dc lie in LDS as
-// plain 256-byte rows; rows that the tap shifts out of their sequence are zero in both.  Both operands of the product
-// have their K along the rows, so fragments are read transposed (ds_read_b64_tr_b16).  4 waves of 64 ci x 64 co each; the
-// column sums S come from two more matrix instructions per k-step with a fragment of ones.
+// A matrix product whose K runs along the rows: 128 ci x 128 co per tap, 294 912 operations per row at 9 taps against 388
+// bytes read, so it is bound by the matrix cores and by what feeds them.  Sequences follow each other without padding; a
+// 32-row step of a tap is full (no row leaves its sequence), empty (skipped) or mixed (the rows that leave it are cleared in
+// the fragment): 32 bits, computed from the step's first position.  Both operands are read transposed
+// (ds_read_b64_tr_b16) from tiles in LDS.  S comes from the same product: a fragment whose row m is 1 where tap m is inside
+// its sequence.
+//   k_wgrad_ck8_ring: all taps in one workgroup, 32 of the 128 input channels.  The decoded xq rows form a ring: every row is
+//     read and decoded once per chunk whatever the number of taps (decoded per tap, the vector instructions alone took
+//     longer than the product).  8 waves, each 5 taps x 16 ci x 64 co: 80 accumulator registers, 9 fragments for 20 matrix
+//     instructions, the next step's fragments in registers before this step's product begins.
+//   k_wgrad_ck8_tap: one tap and 64 input channels per workgroup, for one tap, for few rows (nine times the workgroups per
+//     row chunk, and every chunk costs a slab of P written and read) and for shifts that no ring in LDS can hold.
 #define CW_TILE 64
-#define CW_IMG (CW_TILE * 256)
+#define CW_DC (CW_TILE * 256)            // bytes of a dc tile
 #define CW_SLAB ((DRK_C + 1) * DRK_C)    // P [128][128], then S [128]
 #define CW_MAX_TAPS 9
 
-// byte offset of 16-byte chunk `ch` of a row: the eight 32-byte pairs of four neighbouring rows fall into different banks
-__device__ __forceinline__ int cw_at(int row, int ch) { return 256 * row + 16 * (ch ^ (((row & 3) << 2) | ((row >> 2) & 3))); }
-__device__ __forceinline__ bf16v8 cw_frag(const char* p0, const char* p1) {
+__device__ __forceinline__ int cw_dc_at(int row, int ch) { return 256 * row + 16 * (ch ^ (((row & 3) << 2) | ((row >> 2) & 3))); }
+__device__ __forceinline__ s16x4 cw_read(const char* p) {
   typedef s16x4 __attribute__((address_space(3))) * lds4;
-  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p0);
-  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p1);
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p);
+}
+__device__ __forceinline__ bf16v8 cw_frag(const char* p0, const char* p1) {
+  const s16x4 lo = cw_read(p0), hi = cw_read(p1);
   return __builtin_bit_cast(bf16v8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-__global__ void __launch_bounds__(256) k_wgrad_ck8(const uint64_t* __restrict__ codes, const unsigned char* __restrict__ exps,
-                                                   const char* __restrict__ dc, float* __restrict__ slabs, long M, int L, int taps,
-                                                   int dil, int tiles_per_wg, int total_tiles) {
-  __shared__ __attribute__((aligned(16))) char smem[2 * CW_IMG];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, wr = w >> 1, wc = w & 1;
-  const int t = blockIdx.y;
-  const long off = (long)(t - taps / 2) * dil;
-  const int T0 = blockIdx.x * tiles_per_wg, T1 = T0 + tiles_per_wg < total_tiles ? T0 + tiles_per_wg : total_tiles;
-  const int srow = tid >> 4, scol = tid & 15;
-  const int kg = lane >> 4, q = (lane >> 2) & 3, p = lane & 3;
-  f32x4 acc[4][4], accs[2];
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+// Bit k: row k of 32 rows that follow each other from position lb of a sequence of L (then the next sequences') is inside
+// its sequence after a shift of o, |o| <= L.
+__device__ __forceinline__ unsigned cw_inside(int lb, int L, int o) {
+  unsigned rows = 0;
+  for (int s = -lb; s < 32; s += L) {                      // a sequence's rows are k = s .. s + L - 1
+    const int lo = max(s + max(-o, 0), 0), n = min(s + min(L - o, L), 32) - lo;
+    rows |= n > 0 ? (~0u >> (32 - n)) << lo : 0u;
+  }
+  return rows;
+}
+// eight bits -> eight halves of all ones or zeros
+__device__ __forceinline__ u32x4 cw_mask(unsigned bits) {
+  u32x4 m;
 #pragma unroll
-  for (int m = 0; m < 4; ++m)
+  for (int d = 0; d < 4; ++d) {
+    const unsigned a = (unsigned)((int)(bits << (31 - 2 * d)) >> 31), b = (unsigned)((int)(bits << (30 - 2 * d)) >> 31);
+    m[d] = (a & 0xffffu) | (b & 0xffff0000u);
+  }
+  return m;
+}
+
+struct CwArgs {
+  const uint64_t* codes;
+  const unsigned char* exps;
+  const char* dc;
+  float* slabs;
+  long M;
+  int L, taps, dil, tiles_per_wg, total_tiles, chunks;
+};
+
+// What a chunk of rows is to a kernel: its first row, its tiles, and where its first row stands in its sequence.
+struct CwChunk {
+  long r0;
+  int nt, lb;
+};
+__device__ __forceinline__ CwChunk cw_chunk(const CwArgs& a, int chunk) {
+  const int T0 = chunk * a.tiles_per_wg;
+  CwChunk c;
+  c.r0 = (long)T0 * CW_TILE;
+  c.nt = (T0 + a.tiles_per_wg < a.total_tiles ? T0 + a.tiles_per_wg : a.total_tiles) - T0;
+  c.lb = (int)(c.r0 % a.L);
+  return c;
+}
+__device__ __forceinline__ int cw_shift(const CwArgs& a, int tap) {      // at most L either way: nothing is inside there
+  const long o = (long)(tap - a.taps / 2) * a.dil;
+  return (int)(o > a.L ? a.L : o < -a.L ? -a.L : o);
+}
+__device__ __forceinline__ bf16v8 cw_clear(bf16v8 f, u32x4 mask) { return __builtin_bit_cast(bf16v8, __builtin_bit_cast(u32x4, f) & mask); }
+
+__global__ void __launch_bounds__(256) k_wgrad_ck8_tap(CwArgs a) {
+  __shared__ __attribute__((aligned(16))) char xs[2][CW_TILE * 128];      // xq, 64 channels
+  __shared__ __attribute__((aligned(16))) char ds[2][CW_DC];
+  // the two halves of a chunk read the same dc: 8 workgroups apart they run on the same XCD
+  const int half = (blockIdx.x >> 3) & 1, chunk = (blockIdx.x >> 4) * 8 + (blockIdx.x & 7);
+  if (chunk >= a.chunks) return;
+  const int tid = threadIdx.x, lane = tid & 63, tap = blockIdx.y, L = a.L;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6), ciq = w >> 1, coh = w & 1;
+  const CwChunk c = cw_chunk(a, chunk);
+  const long g0 = c.r0 + (long)(tap - a.taps / 2) * a.dil;
+  const int shift = cw_shift(a, tap), lstep = 32 % L;
+  int lb = c.lb;
+  uint64_t rq[2];
+  unsigned re[2];
+  f32x4 rd[4];
+  auto fetch = [&](int T) __attribute__((always_inline)) {
 #pragma unroll
-    for (int n = 0; n < 4; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-  accs[0] = accs[1] = f32x4{0.f, 0.f, 0.f, 0.f};
-  bf16v8 one;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) one[i] = (__bf16)1.f;
-  for (int T = T0; T < T1; ++T) {
-    __syncthreads();
+    for (int i = 0; i < 2; ++i) {
+      const int it = tid + 256 * i;
+      const long g = g0 + 64L * T + (it >> 3);
+      rq[i] = 0;
+      re[i] = 0;
+      if (g >= 0 && g < a.M) {
+        rq[i] = a.codes[g * (DRK_C / 8) + 8 * half + (it & 7)];
+        re[i] = a.exps[g * CK_EXPS + 2 * half + ((it >> 2) & 1)];
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const long r = (long)T * CW_TILE + srow + 16 * i;
-      const int at = cw_at(srow + 16 * i, scol);
-      f32x4 dv = {0.f, 0.f, 0.f, 0.f};
-      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (r < M) {
-        const long l = r % L + off;
-        if (l >= 0 && l < L) {
-          dv = *(const f32x4*)(dc + r * 256 + 16 * scol);
-          decode8(codes[(r + off) * (DRK_C / 8) + scol], exps[(r + off) * CK_EXPS + (scol >> 2)], v);
-        }
-      }
-      store8_bf16(smem + at, v);
-      *(f32x4*)(smem + CW_IMG + at) = dv;
+      const int it = tid + 256 * i;
+      const long g = c.r0 + 64L * T + (it >> 4);
+      rd[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (g < a.M) rd[i] = *(const f32x4*)(a.dc + g * 256 + 16 * (it & 15));
     }
-    __syncthreads();
+  };
+  auto store = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int it = tid + 256 * i, row = it >> 3;
+      float v[8];
+      decode8(rq[i], re[i], v);
+      store8_bf16(xs[buf] + 128 * row + 16 * ((it & 7) ^ (((row >> 1) & 1) << 1) ^ (((row >> 3) & 1) << 2)), v);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int it = tid + 256 * i;
+      *(f32x4*)(ds[buf] + cw_dc_at(it >> 4, it & 15)) = rd[i];
+    }
+  };
+  // lane 16 kg + 4 q + p asks for row 8 kg + q (+ 4 in the second read), columns 4 p .. 4 p + 3 of a 16-channel tile.  The
+  // 32-byte pairs of an xq row are exchanged by bits 1 and 3 of the row: 8 rows of 32 lanes fall into different banks.
+  const int kg = lane >> 4, q = (lane >> 2) & 3, p = lane & 3, row = 8 * kg + q;
+  const int aoff = 128 * row + 32 * ((2 * ciq) ^ ((row >> 1) & 1) ^ ((row >> 2) & 2)) + 16 * (p >> 1) + 8 * (p & 1);
+  const int boff = cw_dc_at(row, 8 * coh + (p >> 1)) + 8 * (p & 1);
+  f32x4 acc[2][4], accs[2];
+#pragma unroll
+  for (int n = 0; n < 4; ++n) acc[0][n] = acc[1][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  accs[0] = accs[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  fetch(0);
+  store(0);
+  __syncthreads();
+  for (int T = 0; T < c.nt; ++T) {
+    if (T + 1 < c.nt) fetch(T + 1);
+    const char *xt = xs[T & 1], *dt = ds[T & 1];
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      bf16v8 af[4], bf[4];
-      const int row = 32 * ks + 8 * kg + q;
+      const unsigned rows = cw_inside(lb, L, shift);
+      if (rows) {
+        bf16v8 af[2], bf[4];
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        af[m] = cw_frag(smem + cw_at(row, 2 * (4 * wr + m) + (p >> 1)) + 8 * (p & 1), smem + cw_at(row + 4, 2 * (4 * wr + m) + (p >> 1)) + 8 * (p & 1));
-        bf[m] = cw_frag(smem + CW_IMG + cw_at(row, 2 * (4 * wc + m) + (p >> 1)) + 8 * (p & 1),
-                        smem + CW_IMG + cw_at(row + 4, 2 * (4 * wc + m) + (p >> 1)) + 8 * (p & 1));
+        for (int n = 0; n < 4; ++n) bf[n] = cw_frag(dt + 8192 * ks + (boff ^ (32 * n)), dt + 8192 * ks + 1024 + (boff ^ (32 * n) ^ 16));
+#pragma unroll
+        for (int m = 0; m < 2; ++m) af[m] = cw_frag(xt + 4096 * ks + (aoff ^ (32 * m)), xt + 4096 * ks + 512 + (aoff ^ (32 * m)));
+        u32x4 mask = cw_mask(rows >> (8 * kg));
+        af[0] = cw_clear(af[0], mask);
+        af[1] = cw_clear(af[1], mask);
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int n = 0; n < 4; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af[m], bf[n], acc[m][n], 0, 0, 0);
+        if (half == 0) {
+          mask &= 0x3f803f80u;                             // ones in the rows that count
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+            accs[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16v8, mask), ciq ? bf[2 + n] : bf[n], accs[n], 0, 0, 0);
+        }
       }
-#pragma unroll
-      for (int m = 0; m < 4; ++m)
-#pragma unroll
-        for (int n = 0; n < 4; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af[m], bf[n], acc[m][n], 0, 0, 0);
-#pragma unroll
-      for (int n = 0; n < 2; ++n) accs[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(one, wr ? bf[2 + n] : bf[n], accs[n], 0, 0, 0);
+      lb += lstep;
+      lb -= lb >= L ? L : 0;
     }
+    if (T + 1 < c.nt) store((T + 1) & 1);                  // its last readers passed the previous barrier
+    __syncthreads();
   }
-  // D[row 4 g + i][col n] of tile (m, n): ci = 64 wr + 16 m + 4 g + i, co = 64 wc + 16 n + (lane & 15)
-  float* dst = slabs + ((long)blockIdx.x * taps + t) * CW_SLAB;
+  // D[row 4 g + v][col] of tile (m, n): ci = 64 half + 32 ciq + 16 m + 4 g + v, co = 64 coh + 16 n + (lane & 15)
+  float* dst = a.slabs + ((long)chunk * a.taps + tap) * CW_SLAB;
   const int g = lane >> 4, cn = lane & 15;
 #pragma unroll
-  for (int m = 0; m < 4; ++m)
+  for (int m = 0; m < 2; ++m)
 #pragma unroll
     for (int n = 0; n < 4; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) dst[(64 * wr + 16 * m + 4 * g + i) * DRK_C + 64 * wc + 16 * n + cn] = acc[m][n][i];
-  if (g == 0) {
+      for (int v = 0; v < 4; ++v) dst[(64 * half + 32 * ciq + 16 * m + 4 * g + v) * DRK_C + 64 * coh + 16 * n + cn] = acc[m][n][v];
+  if (half == 0 && g == 0) {
 #pragma unroll
-    for (int n = 0; n < 2; ++n) dst[DRK_C * DRK_C + 64 * wc + 16 * (2 * wr + n) + cn] = accs[n][0];
+    for (int n = 0; n < 2; ++n) dst[DRK_C * DRK_C + 64 * coh + 16 * (2 * ciq + n) + cn] = accs[n][0];
   }
 }
 
-// dwt[t][ci][co] += gamma[ci] * sum of P + beta[ci] * sum of S over the chunks, in order (gamma null: 1 and 0)
-__global__ void __launch_bounds__(256) k_wgrad_ck8_join(const float* __restrict__ slabs, int chunks, int taps,
-                                                        const float* __restrict__ gamma, const float* __restrict__ beta,
-                                                        float* __restrict__ dwt) {
-  const int t = blockIdx.y, ci = blockIdx.x * 8 + (threadIdx.x >> 5), c4 = 4 * (threadIdx.x & 31);
-  f32x4 P = {0.f, 0.f, 0.f, 0.f}, S = P;
-  for (int k = 0; k < chunks; ++k) {
-    const float* s = slabs + ((long)k * taps + t) * CW_SLAB;
-    P += *(const f32x4*)(s + ci * DRK_C + c4);
-    if (gamma) S += *(const f32x4*)(s + DRK_C * DRK_C + c4);
+#define CW_NT 5                           // taps of a wave: every second one
+#define CW_RING_MAX 1024                  // rows
+#define CW_RD 288                         // bytes of a dc row: 32 more than it holds, so that 8 rows of 32 bytes meet no bank twice
+#define CW_RDC (CW_TILE * CW_RD)
+// Ring blocks of 64 rows: those a tile reads, one more for the next tile's first step, one that is being filled.
+__host__ __device__ static inline int cw_ring_rows(int taps, int dilation) {
+  const int need = (((taps - 1) * dilation + 63) / 64 + 3) * 64;
+  int r = 256;
+  while (r < need) r *= 2;
+  return r;
+}
+#define CW_RING_LDS(rows) (((rows) + 16) * 64 + 3 * CW_RDC)      // (the ring's first 16 rows once more behind its last)
+
+// K slot 8 kg + j of a 32-row step is row 4 kg + j (j < 4) or 12 + 4 kg + j: the rows that 32 lanes read together follow each
+// other.  32 row bits -> the eight of a lane's slots.
+__device__ __forceinline__ unsigned cw_slots(unsigned rows, int kg) {
+  return ((rows >> (4 * kg)) & 15u) | ((rows >> (16 + 4 * kg)) & 15u) << 4;
+}
+
+__global__ void __launch_bounds__(512) k_wgrad_ck8_ring(CwArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];              // the ring, then three dc tiles
+  typedef s16x4 __attribute__((address_space(3))) * lds4;
+  // the four quarters of a chunk read the same dc: 8 workgroups apart they run on the same XCD
+  const int quarter = (blockIdx.x >> 3) & 3, chunk = (blockIdx.x >> 5) * 8 + (blockIdx.x & 7);
+  if (chunk >= a.chunks) return;
+  const int tid = threadIdx.x, lane = tid & 63, L = a.L, jn = a.taps;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6), tg = w >> 2, cih = (w >> 1) & 1, coh = w & 1;
+  const CwChunk c = cw_chunk(a, chunk);
+  const int span = (jn - 1) * a.dil, sb = (span + 63) / 64;                // a tile reads ring blocks T .. T + sb
+  const int R = cw_ring_rows(jn, a.dil), bwrap = R / 64 - 1;
+  const unsigned wrap = 64u * R - 1u;
+  const long g0 = c.r0 - (long)(jn / 2) * a.dil;                          // the ring's first row
+  const int dcs = (R + 16) * 64;
+
+  // staging: 256 threads an xq block (row tid / 4, 8 channels), all of them a dc tile (rows tid / 16 and + 32).  The halves
+  // of a ring row are exchanged by bit 2 of the row: the 8 rows of 32 lanes fall into different banks wherever they start.
+  const int xrow = (tid & 255) >> 2, xch = tid & 3;
+  const uint64_t* const xc = a.codes + 4 * quarter + xch;
+  const unsigned char* const xe = a.exps + quarter;
+  const int xput = 64 * xrow + 16 * (xch ^ (((xrow >> 2) & 1) << 1)), dput = dcs + (tid >> 4) * CW_RD + 16 * (tid & 15);
+  auto fetch_x = [&](int b, uint64_t& q, unsigned& e) __attribute__((always_inline)) {
+    const long g = g0 + 64L * b + xrow;
+    const bool on = g >= 0 && g < a.M;
+    q = on ? xc[g * (DRK_C / 8)] : 0;
+    e = on ? xe[g * CK_EXPS] : 0;
+  };
+  auto store_x = [&](int b, uint64_t q, unsigned e) __attribute__((always_inline)) {
+    float v[8];
+    decode8(q, e, v);
+    bf16v8 o;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = (__bf16)v[i];
+    *(bf16v8*)(smem + (b & bwrap) * 4096 + xput) = o;
+    if ((b & bwrap) == 0 && xrow < 16) *(bf16v8*)(smem + 64 * R + xput) = o;
+  };
+  const char* dp = a.dc + (c.r0 + (tid >> 4)) * 256 + 16 * (tid & 15);    // of the next tile to be read
+  long left = a.M - c.r0 - (tid >> 4);                                     // rows from there to the end
+  auto fetch_d = [&](f32x4 d[2]) __attribute__((always_inline)) {
+    d[0] = d[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (left > 0) d[0] = *(const f32x4*)dp;
+    if (left > 32) d[1] = *(const f32x4*)(dp + 32 * 256);
+    dp += CW_DC;
+    left -= CW_TILE;
+  };
+  auto store_d = [&](int buf, const f32x4 d[2]) __attribute__((always_inline)) {
+    *(f32x4*)(smem + buf * CW_RDC + dput) = d[0];
+    *(f32x4*)(smem + buf * CW_RDC + dput + 32 * CW_RD) = d[1];
+  };
+
+  // fragments: lane 16 kg + 4 q + p asks for row 4 kg + q (+ 16 in the second read), columns 4 p .. 4 p + 3 of a 16-channel tile
+  const int kg = lane >> 4, q = (lane >> 2) & 3, p = lane & 3;
+  unsigned aoff[CW_NT];
+  int shift[CW_NT];
+#pragma unroll
+  for (int i = 0; i < CW_NT; ++i) {
+    const int j = tg + 2 * i < jn ? tg + 2 * i : jn - 1;    // (a wave without a fifth tap reads where another one does)
+    shift[i] = tg + 2 * i < jn ? cw_shift(a, j) : L;
+    const int row = j * a.dil + 4 * kg + q;
+    aoff[i] = 64 * row + 32 * (cih ^ ((row >> 2) & 1)) + 8 * p;
   }
-  f32x4* o = (f32x4*)(dwt + ((long)t * DRK_C + ci) * DRK_C + c4);
-  *o += gamma ? P * gamma[ci] + S * beta[ci] : P;
+  const unsigned boff = dcs + (4 * kg + q) * CW_RD + 128 * coh + 8 * p;
+  struct Frags { bf16v8 a[CW_NT], b[4]; };
+  // (addresses are offsets into LDS: smem is all that this kernel has there, so it starts at 0)
+  auto frag = [&](unsigned at, int second) __attribute__((always_inline)) {
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)at);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)(at + second));
+    return __builtin_bit_cast(bf16v8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  auto load = [&](Frags& f, int T, int buf, int ks) __attribute__((always_inline)) {
+    const unsigned at = boff + buf * CW_RDC, base = (unsigned)T * 4096u + 2048u * ks;      // (base: modulo 2^32, a multiple of the ring)
+#pragma unroll
+    for (int n = 0; n < 4; ++n) f.b[n] = frag(at + 32 * ks * CW_RD + 32 * n, 16 * CW_RD);
+#pragma unroll
+    for (int i = 0; i < CW_NT; ++i) f.a[i] = frag((base + aoff[i]) & wrap, 16 * 64);
+  };
+
+  f32x4 acc[CW_NT][4], accs = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < CW_NT; ++i)
+#pragma unroll
+    for (int n = 0; n < 4; ++n) acc[i][n] = accs;
+  const int my_tap = lane & 15, my_shift = cw_shift(a, my_tap), o_first = cw_shift(a, 0), o_last = cw_shift(a, jn - 1);
+  const unsigned ones = my_tap < jn ? 0x3f803f80u : 0u;
+  const int lstep = 32 % L;
+  int lb = c.lb;
+  auto step = [&](Frags& f) __attribute__((always_inline)) {
+    unsigned rows[CW_NT], mine = ~0u;
+    if (lb + 31 < L && lb + o_first >= 0 && lb + 31 + o_last < L) {       // every row inside its sequence at every tap
+#pragma unroll
+      for (int i = 0; i < CW_NT; ++i) rows[i] = shift[i] < L ? ~0u : 0u;
+    } else {
+      mine = cw_inside(lb, L, my_shift);                   // lane t finds tap t's rows
+      unsigned cut = 0;
+#pragma unroll
+      for (int i = 0; i < CW_NT; ++i) {
+        rows[i] = shift[i] < L ? __builtin_amdgcn_readlane(mine, tg + 2 * i) : 0u;
+        cut |= rows[i] ^ (unsigned)-(int)(rows[i] & 1u);   // neither all nor none
+      }
+      if (cut) {
+#pragma unroll
+        for (int i = 0; i < CW_NT; ++i) f.a[i] = cw_clear(f.a[i], cw_mask(cw_slots(rows[i], kg)));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < CW_NT; ++i)
+      if (rows[i]) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) acc[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.a[i], f.b[n], acc[i][n], 0, 0, 0);
+      }
+    if (quarter == 0) {                                    // wave (tg, cih) sums co tile 2 tg + cih of its half
+      u32x4 v = cw_mask(cw_slots(mine, kg));
+      v &= ones;
+      accs = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16v8, v), tg ? (cih ? f.b[3] : f.b[2]) : (cih ? f.b[1] : f.b[0]), accs, 0, 0, 0);
+    }
+    lb += lstep;
+    lb -= lb >= L ? L : 0;
+  };
+
+  {
+    f32x4 d0[2], d1[2];
+    fetch_d(d0);
+    fetch_d(d1);                                           // (past the chunk's end: rows that no step multiplies)
+#pragma unroll 1
+    for (int b = tid >> 8; b < sb + 2; b += 8) {           // two blocks at a time, four times in flight
+      uint64_t xq[4];
+      unsigned xs[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) fetch_x(b + 2 * u, xq[u], xs[u]);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (b + 2 * u < sb + 2) store_x(b + 2 * u, xq[u], xs[u]);
+    }
+    store_d(0, d0);
+    store_d(1, d1);
+  }
+  __syncthreads();
+  // What tile T + 2 needs is stored at the end of tile T; it was requested at the start of tile T - 1.
+  struct Staged { f32x4 d[2]; uint64_t q; unsigned e; };
+  auto request = [&](Staged& s, int T) __attribute__((always_inline)) {
+    fetch_d(s.d);
+    if (tid < 256) fetch_x(T + sb, s.q, s.e);
+  };
+  Frags f0, f1;
+  load(f0, 0, 0, 0);
+  int buf = 0;                                             // T mod 3
+  auto tile = [&](int T, Staged& now, Staged& later) __attribute__((always_inline)) {
+    const int nbuf = buf == 2 ? 0 : buf + 1, fbuf = buf == 0 ? 2 : buf - 1;
+    request(later, T + 3);                                 // (past the chunk's end: stored, and not used)
+    load(f1, T, buf, 1);
+    step(f0);
+    load(f0, T + 1, nbuf, 0);
+    step(f1);
+    store_d(fbuf, now.d);                                  // the buffer and the block whose last readers passed the previous barrier
+    if (tid < 256) store_x(T + 2 + sb, now.q, now.e);
+    buf = nbuf;
+    __syncthreads();
+  };
+  Staged s0, s1;
+  request(s0, 2);
+  for (int T = 0; T < c.nt; T += 2) {
+    tile(T, s0, s1);
+    if (T + 1 < c.nt) tile(T + 1, s1, s0);
+  }
+
+  // D[row 4 g + v][col] of tile n: ci = 32 quarter + 16 cih + 4 g + v, co = 64 coh + 16 n + (lane & 15)
+  const int g = lane >> 4, cn = lane & 15;
+#pragma unroll
+  for (int i = 0; i < CW_NT; ++i) {
+    if (tg + 2 * i >= jn) continue;
+    float* dst = a.slabs + ((long)chunk * jn + tg + 2 * i) * CW_SLAB;
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) dst[(32 * quarter + 16 * cih + 4 * g + v) * DRK_C + 64 * coh + 16 * n + cn] = acc[i][n][v];
+  }
+  if (quarter == 0) {
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+      if (4 * g + v < jn) a.slabs[((long)chunk * jn + 4 * g + v) * CW_SLAB + DRK_C * DRK_C + 64 * coh + 16 * (2 * tg + cih) + cn] = accs[v];
+  }
+}
+
+// dwt[t][ci][co] += gamma[ci] * sum of P + beta[ci] * sum of S over the chunks (gamma null: 1 and 0).  A workgroup joins 4
+// rows of P: eight groups of threads take an eighth of the chunks each, in order, and are then added in order, so that
+// enough loads are in flight to read the slabs at the rate they come from the Infinity Cache.
+__global__ void __launch_bounds__(1024) k_wgrad_ck8_join(const float* __restrict__ slabs, int chunks, int taps,
+                                                         const float* __restrict__ gamma, const float* __restrict__ beta,
+                                                         float* __restrict__ dwt) {
+  __shared__ f32x4 lp[8][4][32], ls[8][32];
+  const int col = threadIdx.x & 31, sub = (threadIdx.x >> 5) & 3, grp = threadIdx.x >> 7;
+  const int t = blockIdx.y, ci = blockIdx.x * 4 + sub, per = (chunks + 7) / 8;
+  const int k0 = grp * per, k1 = k0 + per < chunks ? k0 + per : chunks;
+  const long step = (long)taps * CW_SLAB;
+  const float* s = slabs + (long)t * CW_SLAB + 4 * col;
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  f32x4 P = zero, S = zero;
+#pragma unroll 8
+  for (int k = k0; k < k1; ++k) P += *(const f32x4*)(s + k * step + ci * DRK_C);
+  if (gamma && sub == 0) {
+#pragma unroll 8
+    for (int k = k0; k < k1; ++k) S += *(const f32x4*)(s + k * step + DRK_C * DRK_C);
+    ls[grp][col] = S;
+  }
+  lp[grp][sub][col] = P;
+  __syncthreads();
+  if (grp) return;
+  P = S = zero;
+#pragma unroll
+  for (int g = 0; g < 8; ++g) P += lp[g][sub][col];
+  if (gamma) {
+#pragma unroll
+    for (int g = 0; g < 8; ++g) S += ls[g][col];
+    P = P * gamma[ci] + S * beta[ci];
+  }
+  f32x4* o = (f32x4*)(dwt + ((long)t * DRK_C + ci) * DRK_C + 4 * col);
+  *o += P;
 }
 
 // ------------------------------------------------------------------------------------------------ C ABI
@@ -447,21 +768,30 @@ extern "C" int drk_ln_bwd_ck8(const float* dh, const signed char* codes, const u
   return DRK_OK;
 }
 
-// Row chunks per tap: enough workgroups for the 256 CUs, no more, because every chunk costs a slab written and read.
-static void cw_plan(long M, int taps, int* tiles_per_wg, int* chunks) {
+// How the work is cut.  All taps in one workgroup (the ring) or one tap per workgroup; row chunks so that the 256 CUs have a
+// workgroup each, no more, because every chunk costs a slab of P and S per tap written and read.
+#define CW_RING_ROWS 1
+struct CwPlan {
+  bool ring;
+  int tiles_per_wg, chunks, total;
+};
+static CwPlan cw_plan(long M, int taps, int dilation) {
+  CwPlan p;
   const long tiles = (M + CW_TILE - 1) / CW_TILE;
-  long most = 256 / taps;
-  const long tpw = (tiles + most - 1) / most;
-  *tiles_per_wg = (int)tpw;
-  *chunks = (int)((tiles + tpw - 1) / tpw);
+  p.ring = taps > 1 && (long)(taps - 1) * dilation <= CW_RING_MAX - 3 * 64 && M >= CW_RING_ROWS;
+  const long most = p.ring ? 64 : 256 / (2 * taps);
+  const long per = (tiles + most - 1) / most;
+  p.tiles_per_wg = (int)per;
+  p.chunks = (int)((tiles + per - 1) / per);
+  p.total = (int)tiles;
+  return p;
 }
 static bool cw_shape_ok(int taps, int dilation) { return taps >= 1 && taps <= CW_MAX_TAPS && (taps & 1) && dilation >= 0; }
 
-extern "C" long drk_conv_wgrad_ck8_workspace_bytes(int B, int L, int taps) {
+extern "C" long drk_conv_wgrad_ck8_workspace_bytes(int B, int L, int taps, int dilation) {
   if (B <= 0 || L <= 0 || !cw_shape_ok(taps, 0)) return 0;
-  int tpw, chunks;
-  cw_plan((long)B * L, taps, &tpw, &chunks);
-  return (long)chunks * taps * CW_SLAB * (long)sizeof(float);
+  if (dilation < 0) return 0;
+  return (long)cw_plan((long)B * L, taps, dilation).chunks * taps * CW_SLAB * (long)sizeof(float);
 }
 
 extern "C" int drk_conv_wgrad_ck8(const signed char* codes, const unsigned char* exps, const float* gamma, const float* beta,
@@ -470,17 +800,31 @@ extern "C" int drk_conv_wgrad_ck8(const signed char* codes, const unsigned char*
   DRK_SHAPE_GUARD("drk_conv_wgrad_ck8");
   CKCHECK(codes && exps && dc && dwt && !gamma == !beta && cw_shape_ok(taps, dilation), "drk_conv_wgrad_ck8");
   CKCHECK(((uintptr_t)codes & 7) == 0 && aligned16(dc) && aligned16(dwt), "drk_conv_wgrad_ck8 (alignment)");
-  CKCHECK(workspace && aligned16(workspace) && workspace_bytes >= drk_conv_wgrad_ck8_workspace_bytes(B, L, taps),
-          "drk_conv_wgrad_ck8 (workspace: 16-byte aligned, drk_conv_wgrad_ck8_workspace_bytes(B, L, taps) bytes)");
+  CKCHECK(workspace && aligned16(workspace) && workspace_bytes >= drk_conv_wgrad_ck8_workspace_bytes(B, L, taps, dilation),
+          "drk_conv_wgrad_ck8 (workspace: 16-byte aligned, drk_conv_wgrad_ck8_workspace_bytes(B, L, taps, dilation) bytes)");
   const long M = (long)B * L;
-  int tpw, chunks;
-  cw_plan(M, taps, &tpw, &chunks);
-  CKCHECK(M < (1L << 36), "drk_conv_wgrad_ck8 (too many rows)");
+  CKCHECK(M < (1L << 36) && L < (1 << 30), "drk_conv_wgrad_ck8 (too many rows)");
+  const CwPlan pl = cw_plan(M, taps, dilation);
+  const int chunks = pl.chunks;
+  const CwArgs a = {(const uint64_t*)codes, exps, (const char*)dc, (float*)workspace, M, L, taps, dilation, pl.tiles_per_wg, pl.total, chunks};
   hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL(k_wgrad_ck8, dim3((unsigned)chunks, (unsigned)taps), dim3(256), 0, st, (const uint64_t*)codes, exps, (const char*)dc,
-                     (float*)workspace, M, L, taps, dilation, tpw, (int)((M + CW_TILE - 1) / CW_TILE));
+  const unsigned g8 = (unsigned)((chunks + 7) / 8);
+  if (pl.ring) {
+    static std::atomic<unsigned> lds_set[DRK_MAX_DEVICES];      // the kernel may use more than 64 KB of LDS: said once per device
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return drk_set_error(e, "drk_conv_wgrad_ck8(hipGetDevice)");
+    if (dev < 0 || dev >= DRK_MAX_DEVICES || !lds_set[dev].load(std::memory_order_acquire)) {
+      e = hipFuncSetAttribute((const void*)k_wgrad_ck8_ring, hipFuncAttributeMaxDynamicSharedMemorySize, CW_RING_LDS(CW_RING_MAX));
+      if (e != hipSuccess) return drk_set_error(e, "drk_conv_wgrad_ck8(LDS size)");
+      if (dev >= 0 && dev < DRK_MAX_DEVICES) lds_set[dev].store(1u, std::memory_order_release);
+    }
+    hipLaunchKernelGGL(k_wgrad_ck8_ring, dim3(g8 * 32), dim3(512), CW_RING_LDS(cw_ring_rows(taps, dilation)), st, a);
+  } else {
+    hipLaunchKernelGGL(k_wgrad_ck8_tap, dim3(g8 * 16, (unsigned)taps), dim3(256), 0, st, a);
+  }
   DRK_CHECK_LAUNCH();
-  hipLaunchKernelGGL(k_wgrad_ck8_join, dim3(DRK_C / 8, (unsigned)taps), dim3(256), 0, st, (const float*)workspace, chunks, taps, gamma, beta, dwt);
+  hipLaunchKernelGGL(k_wgrad_ck8_join, dim3(DRK_C / 4, (unsigned)taps), dim3(1024), 0, st, (const float*)workspace, chunks, taps, gamma, beta, dwt);
   DRK_CHECK_LAUNCH();
   return DRK_OK;
 }

@@ -838,7 +838,7 @@ def conv_wgrad_ck8(ck, gamma, beta, dc, dwt, dilation):
     if not (1 <= taps <= 9 and taps % 2 == 1) or dilation < 0:
         raise ValueError(f'conv_wgrad_ck8: an odd number of taps up to 9 and dilation >= 0, got {taps}, {dilation}')
     _here('conv_wgrad_ck8', gamma, beta, dc, dwt)
-    need = _lib.load().drk_conv_wgrad_ck8_workspace_bytes(B, L, taps)
+    need = _lib.load().drk_conv_wgrad_ck8_workspace_bytes(B, L, taps, dilation)
     ws = _scratch(need, dc.device)
     _lib.call('drk_conv_wgrad_ck8', codes, exps, _f(gamma, 'gamma'), _f(beta, 'beta'), _b16(dc, 'dc'), _f(dwt, 'dwt'), B, L, taps,
               dilation, _raw(ws), need, _stream())

@@ -397,8 +397,8 @@ int drk_ln_bwd_ck8(const float* dh, const signed char* codes, const unsigned cha
                    float* sums, int B, int L, void* workspace, long workspace_bytes, void* stream);
 /* drk_conv_wgrad_bf16 with the checkpoint in the place of h: dwt[t][ci][co] += sum_rows h[row + (t - taps/2)*dilation][ci] *
  * dc[row][co], h = gamma * xq + beta (gamma, beta NULL: h = xq) and 0 outside the row's sequence; taps odd, <= 9.  Exact
- * products, fp32 sums in a fixed order. */
-long drk_conv_wgrad_ck8_workspace_bytes(int B, int L, int taps);
+ * products, fp32 sums in a fixed order; a NaN or an infinity in dc reaches every tap. */
+long drk_conv_wgrad_ck8_workspace_bytes(int B, int L, int taps, int dilation);
 int drk_conv_wgrad_ck8(const signed char* codes, const unsigned char* exps, const float* gamma, const float* beta,
                        const void* dc, float* dwt, int B, int L, int taps, int dilation, void* workspace,
                        long workspace_bytes, void* stream);
