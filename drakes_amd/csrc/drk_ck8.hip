@@ -270,6 +270,7 @@ __global__ void __launch_bounds__(256) k_ck8_sums(const float* __restrict__ slab
   __shared__ float red[32][8];
   const int c = threadIdx.x & 7, s0 = threadIdx.x >> 3, i = blockIdx.x * 8 + c;
   float s = 0.f;
+#pragma unroll 8
   for (int k = s0; k < n; k += 32) s += slabs[(long)k * (4 * DRK_C) + i];
   red[s0][c] = s;
   for (int w = 16; w > 0; w >>= 1) {
@@ -465,7 +466,7 @@ __global__ void __launch_bounds__(256) k_wgrad_ck8_tap(CwArgs a) {
   }
 }
 
-#define CW_NT 5                           // taps of a wave: every second one
+#define CW_NT 5                           // A fragments of a wave: four taps, and tap 8 for two of the four co tiles
 #define CW_RING_MAX 1024                  // rows
 #define CW_RD 288                         // bytes of a dc row: 32 more than it holds, so that 8 rows of 32 bytes meet no bank twice
 #define CW_RDC (CW_TILE * CW_RD)
@@ -476,14 +477,10 @@ __host__ __device__ static inline int cw_ring_rows(int taps, int dilation) {
   while (r < need) r *= 2;
   return r;
 }
-#define CW_RING_LDS(rows) (((rows) + 16) * 64 + 3 * CW_RDC)      // (the ring's first 16 rows once more behind its last)
+#define CW_RING_LDS(rows) (((rows) + 16) * 64 + 3 * CW_RDC + 128)      // (the ring's first 16 rows once more behind its last)
 
 // K slot 8 kg + j of a 32-row step is row 4 kg + j (j < 4) or 12 + 4 kg + j: the rows that 32 lanes read together follow each
-// other.  32 row bits -> the eight of a lane's slots.
-__device__ __forceinline__ unsigned cw_slots(unsigned rows, int kg) {
-  return ((rows >> (4 * kg)) & 15u) | ((rows >> (16 + 4 * kg)) & 15u) << 4;
-}
-
+// other.
 __global__ void __launch_bounds__(512) k_wgrad_ck8_ring(CwArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];              // the ring, then three dc tiles
   typedef s16x4 __attribute__((address_space(3))) * lds4;
@@ -534,18 +531,19 @@ __global__ void __launch_bounds__(512) k_wgrad_ck8_ring(CwArgs a) {
     *(f32x4*)(smem + buf * CW_RDC + dput + 32 * CW_RD) = d[1];
   };
 
-  // fragments: lane 16 kg + 4 q + p asks for row 4 kg + q (+ 16 in the second read), columns 4 p .. 4 p + 3 of a 16-channel tile
+  // fragments: lane 16 kg + 4 q + p asks for row 4 kg + q (+ 16 in the second read), columns 4 p .. 4 p + 3 of a 16-channel
+  // tile.  Wave (tg, cih, coh) multiplies taps 2 i + tg (i < 4) with the four co tiles of its half, tap 8 with the first two
+  // of b, and the ones of S with b[0]: b's order is such that the waves of a half share tap 8 and S among them.
   const int kg = lane >> 4, q = (lane >> 2) & 3, p = lane & 3;
   unsigned aoff[CW_NT];
-  int shift[CW_NT];
 #pragma unroll
   for (int i = 0; i < CW_NT; ++i) {
-    const int j = tg + 2 * i < jn ? tg + 2 * i : jn - 1;    // (a wave without a fifth tap reads where another one does)
-    shift[i] = tg + 2 * i < jn ? cw_shift(a, j) : L;
-    const int row = j * a.dil + 4 * kg + q;
+    const int t = i < 4 ? 2 * i + tg : 8;
+    const int row = (t < jn ? t : jn - 1) * a.dil + 4 * kg + q;      // (without such a tap: another one's rows, and not stored)
     aoff[i] = 64 * row + 32 * (cih ^ ((row >> 2) & 1)) + 8 * p;
   }
-  const unsigned boff = dcs + (4 * kg + q) * CW_RD + 128 * coh + 8 * p;
+  const int co0 = 2 * tg + cih, co1 = co0 ^ 1, co2 = 2 * (1 - tg);   // b[0], b[1], b[2] (b[3] is the tile after b[2])
+  const unsigned boff = dcs + (4 * kg + q) * CW_RD + 128 * coh + 8 * p, boff0 = boff + 32 * co0, boff1 = boff + 32 * co1, boff2 = boff + 32 * co2;
   struct Frags { bf16v8 a[CW_NT], b[4]; };
   // (addresses are offsets into LDS: smem is all that this kernel has there, so it starts at 0)
   auto frag = [&](unsigned at, int second) __attribute__((always_inline)) {
@@ -554,50 +552,56 @@ __global__ void __launch_bounds__(512) k_wgrad_ck8_ring(CwArgs a) {
     return __builtin_bit_cast(bf16v8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   };
   auto load = [&](Frags& f, int T, int buf, int ks) __attribute__((always_inline)) {
-    const unsigned at = boff + buf * CW_RDC, base = (unsigned)T * 4096u + 2048u * ks;      // (base: modulo 2^32, a multiple of the ring)
-#pragma unroll
-    for (int n = 0; n < 4; ++n) f.b[n] = frag(at + 32 * ks * CW_RD + 32 * n, 16 * CW_RD);
+    const unsigned at = buf * CW_RDC, base = (unsigned)T * 4096u + 2048u * ks;      // (base: modulo 2^32, a multiple of the ring)
+    f.b[0] = frag(at + boff0 + 32 * ks * CW_RD, 16 * CW_RD);
+    f.b[1] = frag(at + boff1 + 32 * ks * CW_RD, 16 * CW_RD);
+    f.b[2] = frag(at + boff2 + 32 * ks * CW_RD, 16 * CW_RD);
+    f.b[3] = frag(at + boff2 + 32 * ks * CW_RD + 32, 16 * CW_RD);
 #pragma unroll
     for (int i = 0; i < CW_NT; ++i) f.a[i] = frag((base + aoff[i]) & wrap, 16 * 64);
   };
+  // the rows of a lane's slots as masks: four bits -> two words, from a table of 16 entries behind the dc tiles
+  const int table = dcs + 3 * CW_RDC;
+  if (tid < 16) *(uint2*)(smem + table + 8 * tid) = make_uint2((tid & 1 ? 0xffffu : 0u) | (tid & 2 ? 0xffff0000u : 0u), (tid & 4 ? 0xffffu : 0u) | (tid & 8 ? 0xffff0000u : 0u));
+  auto mask = [&](unsigned rows) __attribute__((always_inline)) {
+    const uint2 lo = *(const uint2*)(smem + table + 8 * ((rows >> (4 * kg)) & 15u)), hi = *(const uint2*)(smem + table + 8 * ((rows >> (16 + 4 * kg)) & 15u));
+    return u32x4{lo.x, lo.y, hi.x, hi.y};
+  };
 
-  f32x4 acc[CW_NT][4], accs = {0.f, 0.f, 0.f, 0.f};
+  f32x4 acc[4][4], acc8[2], accs = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < CW_NT; ++i)
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int n = 0; n < 4; ++n) acc[i][n] = accs;
+  acc8[0] = acc8[1] = accs;
   const int my_tap = lane & 15, my_shift = cw_shift(a, my_tap), o_first = cw_shift(a, 0), o_last = cw_shift(a, jn - 1);
   const unsigned ones = my_tap < jn ? 0x3f803f80u : 0u;
   const int lstep = 32 % L;
   int lb = c.lb;
-  auto step = [&](Frags& f) __attribute__((always_inline)) {
-    unsigned rows[CW_NT], mine = ~0u;
-    if (lb + 31 < L && lb + o_first >= 0 && lb + 31 + o_last < L) {       // every row inside its sequence at every tap
+  // One step: rows that leave their sequence are cleared, and the next step's fragments (tile T, ks) are requested among this
+  // one's matrix instructions.  There is no branch around a tap that reaches no row: 19 matrix instructions in one piece with
+  // the next step's reads between them took less time than 14 to 16 behind branches.
+  auto step = [&](Frags& f, Frags& next, int T, int buf, int ks) __attribute__((always_inline)) {
+    u32x4 v = {ones, ones, ones, ones};
+    if (!(lb + 31 < L && lb + o_first >= 0 && lb + 31 + o_last < L)) {
+      const unsigned mine = cw_inside(lb, L, my_shift);    // lane t finds tap t's rows
 #pragma unroll
-      for (int i = 0; i < CW_NT; ++i) rows[i] = shift[i] < L ? ~0u : 0u;
-    } else {
-      mine = cw_inside(lb, L, my_shift);                   // lane t finds tap t's rows
-      unsigned cut = 0;
-#pragma unroll
-      for (int i = 0; i < CW_NT; ++i) {
-        rows[i] = shift[i] < L ? __builtin_amdgcn_readlane(mine, tg + 2 * i) : 0u;
-        cut |= rows[i] ^ (unsigned)-(int)(rows[i] & 1u);   // neither all nor none
-      }
-      if (cut) {
-#pragma unroll
-        for (int i = 0; i < CW_NT; ++i) f.a[i] = cw_clear(f.a[i], cw_mask(cw_slots(rows[i], kg)));
-      }
+      for (int i = 0; i < CW_NT; ++i) f.a[i] = cw_clear(f.a[i], mask(__builtin_amdgcn_readlane(mine, i < 4 ? 2 * i + tg : 8)));
+      v &= mask(mine);
     }
+    load(next, T, buf, ks);
 #pragma unroll
-    for (int i = 0; i < CW_NT; ++i)
-      if (rows[i]) {
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int n = 0; n < 4; ++n) acc[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.a[i], f.b[n], acc[i][n], 0, 0, 0);
-      }
-    if (quarter == 0) {                                    // wave (tg, cih) sums co tile 2 tg + cih of its half
-      u32x4 v = cw_mask(cw_slots(mine, kg));
-      v &= ones;
-      accs = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16v8, v), tg ? (cih ? f.b[3] : f.b[2]) : (cih ? f.b[1] : f.b[0]), accs, 0, 0, 0);
+      for (int n = 0; n < 4; ++n) acc[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.a[i], f.b[n], acc[i][n], 0, 0, 0);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) acc8[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.a[4], f.b[n], acc8[n], 0, 0, 0);
+    accs = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16v8, v), f.b[0], accs, 0, 0, 0);
+#pragma unroll
+    for (int u = 0; u < 18; ++u) {                         // (a matrix instruction takes 16 cycles, its issue 4)
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
     lb += lstep;
     lb -= lb >= L ? L : 0;
@@ -633,10 +637,8 @@ __global__ void __launch_bounds__(512) k_wgrad_ck8_ring(CwArgs a) {
   auto tile = [&](int T, Staged& now, Staged& later) __attribute__((always_inline)) {
     const int nbuf = buf == 2 ? 0 : buf + 1, fbuf = buf == 0 ? 2 : buf - 1;
     request(later, T + 3);                                 // (past the chunk's end: stored, and not used)
-    load(f1, T, buf, 1);
-    step(f0);
-    load(f0, T + 1, nbuf, 0);
-    step(f1);
+    step(f0, f1, T, buf, 1);
+    step(f1, f0, T + 1, nbuf, 0);
     store_d(fbuf, now.d);                                  // the buffer and the block whose last readers passed the previous barrier
     if (tid < 256) store_x(T + 2 + sb, now.q, now.e);
     buf = nbuf;
@@ -649,21 +651,23 @@ __global__ void __launch_bounds__(512) k_wgrad_ck8_ring(CwArgs a) {
     if (T + 1 < c.nt) tile(T + 1, s1, s0);
   }
 
-  // D[row 4 g + v][col] of tile n: ci = 32 quarter + 16 cih + 4 g + v, co = 64 coh + 16 n + (lane & 15)
+  // D[row 4 g + v][col]: ci = 32 quarter + 16 cih + 4 g + v, co = 64 coh + 16 (the fragment's co tile) + (lane & 15)
   const int g = lane >> 4, cn = lane & 15;
+  const int co[4] = {16 * co0, 16 * co1, 16 * co2, 16 * co2 + 16};
 #pragma unroll
   for (int i = 0; i < CW_NT; ++i) {
-    if (tg + 2 * i >= jn) continue;
-    float* dst = a.slabs + ((long)chunk * jn + tg + 2 * i) * CW_SLAB;
+    const int t = i < 4 ? 2 * i + tg : 8;
+    if (t >= jn) continue;
+    float* dst = a.slabs + ((long)chunk * jn + t) * CW_SLAB + (32 * quarter + 16 * cih + 4 * g) * DRK_C + 64 * coh + cn;
 #pragma unroll
-    for (int n = 0; n < 4; ++n)
+    for (int n = 0; n < (i < 4 ? 4 : 2); ++n)
 #pragma unroll
-      for (int v = 0; v < 4; ++v) dst[(32 * quarter + 16 * cih + 4 * g + v) * DRK_C + 64 * coh + 16 * n + cn] = acc[i][n][v];
+      for (int v = 0; v < 4; ++v) dst[v * DRK_C + co[n]] = i < 4 ? acc[i][n][v] : acc8[n & 1][v];
   }
   if (quarter == 0) {
 #pragma unroll
     for (int v = 0; v < 4; ++v)
-      if (4 * g + v < jn) a.slabs[((long)chunk * jn + 4 * g + v) * CW_SLAB + DRK_C * DRK_C + 64 * coh + 16 * (2 * tg + cih) + cn] = accs[v];
+      if (4 * g + v < jn) a.slabs[((long)chunk * jn + 4 * g + v) * CW_SLAB + DRK_C * DRK_C + 64 * coh + co[0] + cn] = accs[v];
   }
 }
 
@@ -768,9 +772,12 @@ extern "C" int drk_ln_bwd_ck8(const float* dh, const signed char* codes, const u
   return DRK_OK;
 }
 
-// How the work is cut.  All taps in one workgroup (the ring) or one tap per workgroup; row chunks so that the 256 CUs have a
-// workgroup each, no more, because every chunk costs a slab of P and S per tap written and read.
-#define CW_RING_ROWS 1
+// How the work is cut.  All taps in one workgroup (the ring) or one tap per workgroup; row chunks so that every CU has one
+// workgroup of the ring kernel or two of the other, no more, because every chunk costs a slab of P and S per tap written and
+// read (half as many workgroups: 155 us instead of 99 at 262 144 rows; one tap, one against two: 50 and 40 us).
+// From this many rows on the ring is the faster one (9 taps of dilation 1 to 16, 128 channels; ring against one tap per
+// workgroup: 6 400 rows 27 and 23 us, 12 800 rows 30 and 30, 25 600 rows 31 and 43, 262 144 rows 99 and 298).
+#define CW_RING_ROWS 12800
 struct CwPlan {
   bool ring;
   int tiles_per_wg, chunks, total;
@@ -779,7 +786,7 @@ static CwPlan cw_plan(long M, int taps, int dilation) {
   CwPlan p;
   const long tiles = (M + CW_TILE - 1) / CW_TILE;
   p.ring = taps > 1 && (long)(taps - 1) * dilation <= CW_RING_MAX - 3 * 64 && M >= CW_RING_ROWS;
-  const long most = p.ring ? 64 : 256 / (2 * taps);
+  const long most = p.ring ? 64 : 512 / (2 * taps);
   const long per = (tiles + most - 1) / most;
   p.tiles_per_wg = (int)per;
   p.chunks = (int)((tiles + per - 1) / per);

@@ -314,13 +314,10 @@ struct TsList {
 };
 __device__ __forceinline__ bool ts_before(float x, int at, float y, int bt) { return x > y || (x == y && at < bt); }
 
-// The k best of the elements of pieces [c0, c1), which this workgroup's threads walked in steps of T with maxima `mine`.
-// put(i, x, at) receives the i-th best; n, the number found, is returned to every thread.
-template <class D, int T, class Put>
-__device__ __forceinline__ int ts_top(const TsRow<D>& R, int c0, int c1, float mine, int k, TsList* list, unsigned* wave_bound, Put put) {
-  constexpr int E = TsRow<D>::E;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  // the k-th largest of the wave's maxima, rounded down to 16 bits
+// A lower bound of the k-th largest of all elements, from the maxima of T threads: the largest of the waves' k-th largest
+// maxima, rounded down to 16 bits.  Ends with a barrier.
+template <int T>
+__device__ __forceinline__ float ts_bound(float mine, int k, unsigned* wave_bound) {
   const unsigned key = ts_key(mine);
   unsigned bound = 0;
 #pragma unroll
@@ -328,13 +325,22 @@ __device__ __forceinline__ int ts_top(const TsRow<D>& R, int c0, int c1, float m
     const unsigned c = bound | (1u << b);
     if (__popcll(__ballot(key >= c)) >= k) bound = c;
   }
-  if (tid == 0) list->n = 0;
-  if (lane == 0) wave_bound[wave] = bound;
+  if ((threadIdx.x & 63) == 0) wave_bound[threadIdx.x >> 6] = bound;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < T / 64; ++w) bound = wave_bound[w] > bound ? wave_bound[w] : bound;
-  const float least = bound < 0x00800000u ? -INFINITY : ts_unkey(bound);     // (smaller keys are -inf's own, rounded down)
-  for (uint64_t todo = __ballot(key >= bound && mine > -INFINITY); todo; todo &= todo - 1) {
+  return bound < 0x00800000u ? -INFINITY : ts_unkey(bound);       // (smaller keys are -inf's own, rounded down)
+}
+
+// The k best of the elements of pieces [c0, c1), which this workgroup's threads walked in steps of T with maxima `mine`.
+// put(i, x, at) receives the i-th best; n, the number found, is returned to every thread.
+template <class D, int T, class Put>
+__device__ __forceinline__ int ts_top(const TsRow<D>& R, int c0, int c1, float mine, int k, TsList* list, unsigned* wave_bound, Put put) {
+  constexpr int E = TsRow<D>::E;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (tid == 0) list->n = 0;
+  const float least = ts_bound<T>(mine, k, wave_bound);
+  for (uint64_t todo = __ballot(mine >= least && mine > -INFINITY); todo; todo &= todo - 1) {
     const int first = c0 + wave * 64 + (int)__builtin_ctzll(todo);      // the wave reads that thread's pieces together
     for (long c = first + (long)T * lane; c < c1; c += (long)T * 64) {
       float v[E];
@@ -485,51 +491,70 @@ __global__ void __launch_bounds__(T) k_scores_row(TsArgs a) {
 }
 
 #define TS_MAX_SPLITS 64
-// The parts of a row, joined: the sums in the order of the parts (every thread the same), the alternatives by counting
-// for each of the parts' own k best how many of the others come before it.
+// The parts of a row, joined: the sums in the order of the parts (every thread the same), the alternatives from the parts'
+// own k best as in ts_top.
 template <class D>
 __global__ void __launch_bounds__(256) k_scores_join(TsArgs a) {
+  constexpr int MOST = TS_MAX_SPLITS * DRK_TOPK_MAX / 256;
   __shared__ float lx[TS_MAX_SPLITS * DRK_TOPK_MAX];
   __shared__ int lat[TS_MAX_SPLITS * DRK_TOPK_MAX];
   __shared__ ts_acc lv[TS_MAX_SPLITS];
-  __shared__ int found;
+  __shared__ unsigned wave_bound[4];
+  __shared__ int kept;
   const long row = blockIdx.x;
   const int tid = threadIdx.x;
   const TsPart* P = (const TsPart*)a.parts + row * a.splits;
   const float c = a.inv_temp * TS_LOG2E;
   const int total = a.splits * a.k;
-  if (tid == 0) found = 0;
-  __syncthreads();
-  if (tid < a.splits) {
-    lv[tid] = P[tid].v;
-    if (a.k) atomicAdd(&found, P[tid].n);
+  int64_t t = -1;
+  float xt = -INFINITY;
+  if (tid == 0) {
+    kept = 0;
+    t = a.tok[row];
+    xt = ts_token<D>(a, row, t);
   }
-  for (int i = tid; i < total; i += 256) {
-    const int p = i / a.k, j = i % a.k;
-    const bool on = j < P[p].n;
-    lx[i] = on ? P[p].x[j] : -INFINITY;
-    lat[i] = on ? P[p].at[j] : 0x7fffffff;
+  if (tid < a.splits) lv[tid] = P[tid].v;
+  float x[MOST], mine = -INFINITY;
+  int at[MOST];
+#pragma unroll
+  for (int u = 0; u < MOST; ++u) {
+    const int i = tid + 256 * u;
+    x[u] = -INFINITY;
+    at[u] = 0;
+    if (i < total) {
+      const int p = i / a.k, j = i - p * a.k;
+      if (j < P[p].n) {
+        x[u] = P[p].x[j];
+        at[u] = P[p].at[j];
+      }
+    }
+    mine = fmaxf(mine, x[u]);
   }
   __syncthreads();
   ts_acc v = lv[0];
   for (int p = 1; p < a.splits; ++p) v = ts_join(v, lv[p], c);
   const float ls = ts_log_sum(v);
-  if (tid == 0) {
-    const int64_t t = a.tok[row];
-    ts_finish(a, row, v, ls, t, ts_token<D>(a, row, t));
-  }
-  for (int i = tid; i < total; i += 256) {
-    const float x = lx[i];
-    const int at = lat[i];
-    if (x == -INFINITY) continue;
+  if (tid == 0) ts_finish(a, row, v, ls, t, xt);
+  if (a.k == 0) return;
+  const float least = ts_bound<256>(mine, a.k, wave_bound);
+#pragma unroll
+  for (int u = 0; u < MOST; ++u)
+    if (x[u] > -INFINITY && x[u] >= least) {
+      const int p = atomicAdd(&kept, 1);     // (in any order: every entry finds its own place)
+      lx[p] = x[u];
+      lat[p] = at[u];
+    }
+  __syncthreads();
+  const int n = kept;
+  for (int i = tid; i < n; i += 256) {
     int place = 0;
-    for (int o = 0; o < total; ++o) place += ts_before(lx[o], lat[o], x, at);
+    for (int o = 0; o < n; ++o) place += ts_before(lx[o], lat[o], lx[i], lat[i]);
     if (place < a.k) {
-      a.top_ids[row * a.k + place] = at;
-      a.top_logp[row * a.k + place] = ts_logp(x, v, ls, a.inv_temp);
+      a.top_ids[row * a.k + place] = lat[i];
+      a.top_logp[row * a.k + place] = ts_logp(lx[i], v, ls, a.inv_temp);
     }
   }
-  for (int i = found + tid; i < a.k; i += 256) {
+  for (int i = n + tid; i < a.k; i += 256) {
     a.top_ids[row * a.k + i] = -1;
     a.top_logp[row * a.k + i] = -INFINITY;
   }
