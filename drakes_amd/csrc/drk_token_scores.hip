@@ -23,6 +23,8 @@
 // largest such bound can hold an alternative.  Their elements are read again (a few hundred per row), those above the bound
 // are listed, and the k that fewest others precede are the answer.  A row with more equal elements at the bound than the
 // list holds (a constant row) is searched k times instead.
+#include <type_traits>
+
 #include "drk_common.h"
 #include "../../include/drakes_hip.h"
 
@@ -45,6 +47,7 @@ struct ts_f16 {
   static __device__ __forceinline__ T put(float v) { return (_Float16)v; }
 };
 
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 #define TS_LOG2E 1.4426950408889634f
 __device__ __forceinline__ float ts_exp2(float v) { return __builtin_amdgcn_exp2f(v); }
 __device__ __forceinline__ float ts_factor(float d) { return fmaxf(d, -1e20f); }
@@ -64,13 +67,29 @@ __device__ __forceinline__ ts_acc ts_join(ts_acc a, ts_acc b, float c) {
   o.t = (a.t + a.s * ts_factor(da)) * fa + (b.t + b.s * ts_factor(db)) * fb;
   return o;
 }
+// Over the 64 lanes, every lane gets the result: lanes 1, 2, 7, 15 apart by DPP, then rows of 16 and halves by exchange.
+template <class Op>
+__device__ __forceinline__ float ts_wave(float v, Op op) {
+  auto dpp = [](float x, auto ctrl) __attribute__((always_inline)) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(x), decltype(ctrl)::value, 0xF, 0xF, false));
+  };
+  v = op(v, dpp(v, std::integral_constant<int, 0xB1>()));
+  v = op(v, dpp(v, std::integral_constant<int, 0x4E>()));
+  v = op(v, dpp(v, std::integral_constant<int, 0x141>()));
+  v = op(v, dpp(v, std::integral_constant<int, 0x140>()));
+  const u32x2 r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  const u32x2 h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return op(__uint_as_float(h[0]), __uint_as_float(h[1]));
+}
 __device__ __forceinline__ ts_acc ts_join_wave(ts_acc v, float c) {
-#pragma unroll
-  for (int w = 32; w > 0; w >>= 1) {
-    const ts_acc o = {__shfl_xor(v.m, w), __shfl_xor(v.s, w), __shfl_xor(v.t, w)};
-    v = ts_join(v, o, c);
-  }
-  return v;
+  ts_acc o;
+  o.m = ts_wave(v.m, [](float a, float b) { return fmaxf(a, b); });
+  const float d = v.m - ts_ref(o.m), f = ts_exp2(c * d);
+  auto add = [](float a, float b) { return a + b; };
+  o.s = ts_wave(v.s * f, add);
+  o.t = ts_wave((v.t + v.s * ts_factor(d)) * f, add);
+  return o;
 }
 
 struct TsArgs {
@@ -112,7 +131,7 @@ __device__ __forceinline__ float ts_token(const TsArgs& a, long row, int64_t t) 
 #define TS_SMALL_V 64
 // a row's word j in LDS: one pad word after every 64, so that 64 threads at a stride of V words meet few banks twice
 __device__ __forceinline__ int ts_pad(int i) { return i + (i >> 6); }
-#define TS_SMALL_LDS (TS_SMALL_V * 64 + TS_SMALL_V)
+#define TS_SMALL_LDS(V) (65 * (V) * (int)sizeof(float))      // 64 rows and a pad word per 64
 
 // n consecutive rows -> LDS as floats, -inf in columns that a per-row list leaves out.  VEC: the rows are dense and 16-byte
 // aligned (and so is the list, by its own width): whole 16-byte pieces.
@@ -124,12 +143,23 @@ __device__ __forceinline__ void ts_stage(const typename D::T* x, const unsigned 
     struct alignas(16) piece { typename D::T v[E]; };
     struct alignas(E) bytes { unsigned char v[E]; };
     const int whole = total / E;
-    for (int i = lane; i < whole; i += 64) {
-      const piece p = ((const piece*)x)[i];
-      bytes b;
-      if (al) b = ((const bytes*)al)[i];
+    for (int i0 = lane; i0 < whole; i0 += 256) {           // four requests in flight
+      piece p[4];
+      bytes b[4];
 #pragma unroll
-      for (int j = 0; j < E; ++j) lds[ts_pad(E * i) + j] = al && !b.v[j] ? -INFINITY : D::get(p.v[j]);
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + 64 * u < whole ? i0 + 64 * u : i0;
+        p[u] = ((const piece*)x)[i];
+        if (al) b[u] = ((const bytes*)al)[i];
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + 64 * u;
+        if (i < whole) {
+#pragma unroll
+          for (int j = 0; j < E; ++j) lds[ts_pad(E * i) + j] = al && !b[u].v[j] ? -INFINITY : D::get(p[u].v[j]);
+        }
+      }
     }
     for (int i = whole * E + lane; i < total; i += 64) lds[ts_pad(i)] = al && !al[i] ? -INFINITY : D::get(x[i]);
   } else {
@@ -140,6 +170,14 @@ __device__ __forceinline__ void ts_stage(const typename D::T* x, const unsigned 
     }
   }
 }
+// columns j0 .. j0 + 7 of a row in LDS, -inf where `on` has no bit (none beyond V)
+__device__ __forceinline__ void ts_eight(const float* lds, int base, int j0, int V, uint64_t on, float x[8]) {
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+    const float e = lds[ts_pad(base + min(j0 + u, V - 1))];
+    x[u] = (on >> (j0 + u)) & 1 ? e : -INFINITY;
+  }
+}
 // the columns of a list that all rows share, as bits
 __device__ __forceinline__ uint64_t ts_shared_list(const unsigned char* al, int V) {
   const bool on = (int)threadIdx.x < V && (!al || al[threadIdx.x]);
@@ -148,7 +186,7 @@ __device__ __forceinline__ uint64_t ts_shared_list(const unsigned char* al, int 
 
 template <class D, bool VEC>
 __global__ void __launch_bounds__(64) k_scores_small(TsArgs a) {
-  __shared__ float lds[TS_SMALL_LDS];
+  extern __shared__ float lds[];
   const long row0 = (long)blockIdx.x * 64, row = row0 + threadIdx.x;
   const int n = (int)(a.rows - row0 < 64 ? a.rows - row0 : 64), V = a.V, base = threadIdx.x * V;
   const bool own_list = a.allowed && a.allowed_stride;
@@ -159,25 +197,33 @@ __global__ void __launch_bounds__(64) k_scores_small(TsArgs a) {
   if (row >= a.rows) return;
   const float c = a.inv_temp * TS_LOG2E;
   ts_acc v = {-INFINITY, 0.f, 0.f};
-  for (int j = 0; j < V; ++j)
-    if ((on >> j) & 1) v.m = fmaxf(v.m, lds[ts_pad(base + j)]);
+  float x[8];
+  for (int j = 0; j < V; j += 8) {
+    ts_eight(lds, base, j, V, on, x);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v.m = fmaxf(v.m, x[u]);
+  }
   const float r = ts_ref(v.m);
-  for (int j = 0; j < V; ++j)
-    if ((on >> j) & 1) {
-      const float d = lds[ts_pad(base + j)] - r, e = ts_exp2(c * d);
+  for (int j = 0; j < V; j += 8) {
+    ts_eight(lds, base, j, V, on, x);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const float d = x[u] - r, e = ts_exp2(c * d);
       v.s += e;
       v.t = fmaf(e, ts_factor(d), v.t);
     }
+  }
   const float ls = ts_log_sum(v);
   ts_finish(a, row, v, ls, t, t >= 0 && t < V && ((on >> t) & 1) ? lds[ts_pad(base + (int)t)] : -INFINITY);
   for (int i = 0; i < a.k; ++i) {            // the best that is left, and out with it
     float best = -INFINITY;
     int at = -1;
-    for (int j = 0; j < V; ++j)
-      if ((on >> j) & 1) {
-        const float x = lds[ts_pad(base + j)];
-        if (x > best) { best = x; at = j; }
-      }
+    for (int j = 0; j < V; j += 8) {
+      ts_eight(lds, base, j, V, on, x);
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (x[u] > best) { best = x[u]; at = j + u; }
+    }
     a.top_ids[row * a.k + i] = at;
     a.top_logp[row * a.k + i] = at < 0 ? -INFINITY : ts_logp(best, v, ls, a.inv_temp);
     if (at >= 0) lds[ts_pad(base + at)] = -INFINITY;
@@ -230,7 +276,7 @@ __device__ __forceinline__ float ts_hot(const TsBwdArgs& a, long row, const TsRo
 template <class D, bool VEC>
 __global__ void __launch_bounds__(64) k_scores_small_bwd(TsBwdArgs a) {
   constexpr int E = 16 / sizeof(typename D::T);
-  __shared__ float lds[TS_SMALL_LDS];
+  extern __shared__ float lds[];
   const long row0 = (long)blockIdx.x * 64, row = row0 + threadIdx.x;
   const int n = (int)(a.rows - row0 < 64 ? a.rows - row0 : 64), V = a.V, base = threadIdx.x * V;
   const bool own_list = a.allowed && a.allowed_stride;
@@ -239,9 +285,12 @@ __global__ void __launch_bounds__(64) k_scores_small_bwd(TsBwdArgs a) {
   __syncthreads();
   if (row < a.rows) {
     const TsRowGrad g = ts_row_grad(a, row);
-    for (int j = 0; j < V; ++j) {
-      float* p = lds + ts_pad(base + j);
-      *p = (on >> j) & 1 ? ts_dense_grad(*p, g, a.inv_temp) * a.inv_temp : 0.f;
+    for (int j = 0; j < V; j += 8) {
+      float x[8];
+      ts_eight(lds, base, j, V, on, x);
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (j + u < V) lds[ts_pad(base + j + u)] = ts_dense_grad(x[u], g, a.inv_temp) * a.inv_temp;
     }
     if (g.g1 != 0.f) lds[ts_pad(base + (int)g.t)] += g.g1 * a.inv_temp;
     for (int r = 0; r < a.k; ++r) {
@@ -262,42 +311,54 @@ __global__ void __launch_bounds__(64) k_scores_small_bwd(TsBwdArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------- longer rows
-// A row as 16-byte pieces: piece c holds elements [c * E - skew, c * E - skew + E), skew = the row's distance from the
-// 16-byte boundary before it.  The first and the last piece may stick out of the row: they are read element by element.
+// A row as whole 16-byte pieces from its first 16-byte boundary on, and up to E - 1 elements before the first and behind the
+// last of them, which one thread each of the row's first part takes (`edge`).
 template <class D>
 struct TsRow {
   static constexpr int E = 16 / sizeof(typename D::T);
   struct alignas(16) piece { typename D::T v[E]; };
   const typename D::T* x;
   const unsigned char* al;
-  int V, skew, pieces;
+  int V, head, full, tail;      // elements before the pieces, pieces, first element behind them
   __device__ __forceinline__ TsRow(const void* base, const unsigned char* allowed, long row, long row_stride, long allowed_stride, int V_) {
     x = (const typename D::T*)base + row * row_stride;
     al = allowed ? allowed + row * allowed_stride : nullptr;
     V = V_;
-    skew = (int)(((uintptr_t)x & 15) / sizeof(typename D::T));
-    pieces = (int)(((long)V + skew + E - 1) / E);
+    const int skew = (int)(((uintptr_t)x & 15) / sizeof(typename D::T));
+    head = skew ? E - skew : 0;                          // (< V: these kernels take V > 64)
+    full = (V - head) / E;
+    tail = head + full * E;
   }
-  __device__ __forceinline__ bool inside(int c) const { return (c > 0 || skew == 0) && (long)c * E - skew + E <= V; }
-  // the elements of piece c as floats, -inf where no column counts
-  __device__ __forceinline__ void load(int c, float v[E]) const {
-    const int j0 = c * E - skew;
-    if (inside(c)) {
-      const piece p = *(const piece*)(x + j0);
+  __device__ __forceinline__ int edge(int tid) const {
+    return tid < head ? tid : tid >= E && tid - E < V - tail ? tail + tid - E : -1;
+  }
+  __device__ __forceinline__ float one(int j) const { return j >= 0 && (!al || al[j]) ? D::get(x[j]) : -INFINITY; }
+  // pieces c, c + step, ... as floats, -inf where no column counts and in pieces from c1 on (whose place an earlier one is
+  // read from): all requests before the first use.  c < c1.
+  template <int N>
+  __device__ __forceinline__ void load(int c, int step, int c1, float v[N][E]) const {
+    piece p[N];
+    uint64_t b[N];
 #pragma unroll
-      for (int j = 0; j < E; ++j) v[j] = D::get(p.v[j]);
-      if (al) {
-        unsigned char b[E];
-        __builtin_memcpy(b, al + j0, E);
+    for (int u = 0; u < N; ++u) {
+      const int at = head + (c + (long)u * step < c1 ? c + u * step : c) * E;
+      p[u] = *(const piece*)(x + at);
+      if (al) __builtin_memcpy(&b[u], al + at, E);
+    }
 #pragma unroll
-        for (int j = 0; j < E; ++j) v[j] = b[j] ? v[j] : -INFINITY;
-      }
-    } else {
+    for (int u = 0; u < N; ++u) {
+      const bool on = c + (long)u * step < c1;
 #pragma unroll
-      for (int j = 0; j < E; ++j) v[j] = j0 + j >= 0 && j0 + j < V && (!al || al[j0 + j]) ? D::get(x[j0 + j]) : -INFINITY;
+      for (int j = 0; j < E; ++j) v[u][j] = on && (!al || ((b[u] >> (8 * j)) & 255)) ? D::get(p[u].v[j]) : -INFINITY;
     }
   }
 };
+// The pieces of a part of a row, and whether the row's edges are among it.
+__device__ __forceinline__ void ts_part(int full, int splits, int per_part, int part, int* c0, int* c1) {
+  const long lo = (long)part * per_part, hi = lo + per_part;
+  *c0 = (int)(lo < full ? lo : full);
+  *c1 = (int)(part == splits - 1 || hi > full ? full : hi);
+}
 
 // floats as unsigned integers of the same order (no NaN among them)
 __device__ __forceinline__ unsigned ts_key(float v) {
@@ -306,6 +367,7 @@ __device__ __forceinline__ unsigned ts_key(float v) {
 }
 __device__ __forceinline__ float ts_unkey(unsigned k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
+#define TS_BATCH 4              // pieces that a thread requests before it uses the first
 #define TS_LIST 512
 struct TsList {
   int n;
@@ -332,28 +394,56 @@ __device__ __forceinline__ float ts_bound(float mine, int k, unsigned* wave_boun
   return bound < 0x00800000u ? -INFINITY : ts_unkey(bound);       // (smaller keys are -inf's own, rounded down)
 }
 
-// The k best of the elements of pieces [c0, c1), which this workgroup's threads walked in steps of T with maxima `mine`.
-// put(i, x, at) receives the i-th best; n, the number found, is returned to every thread.
-template <class D, int T, class Put>
-__device__ __forceinline__ int ts_top(const TsRow<D>& R, int c0, int c1, float mine, int k, TsList* list, unsigned* wave_bound, Put put) {
+// The k best of the elements of pieces [c0, c1), which this workgroup's threads walked in steps of T, and of the threads' own
+// `xe` at column je (-inf: none); mine: a thread's maximum of all; ONE: x holds all of a thread's pieces (one batch).
+// put(i, x, at) receives the i-th best; the number found is returned to every thread.
+template <class D, int T, bool ONE, class Put>
+__device__ __forceinline__ int ts_top(const TsRow<D>& R, int c0, int c1, const float (&x)[TS_BATCH][TsRow<D>::E], float xe, int je,
+                                      float mine, int k, TsList* list, unsigned* wave_bound, Put put) {
   constexpr int E = TsRow<D>::E;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (tid == 0) list->n = 0;
   const float least = ts_bound<T>(mine, k, wave_bound);
-  for (uint64_t todo = __ballot(mine >= least && mine > -INFINITY); todo; todo &= todo - 1) {
-    const int first = c0 + wave * 64 + (int)__builtin_ctzll(todo);      // the wave reads that thread's pieces together
-    for (long c = first + (long)T * lane; c < c1; c += (long)T * 64) {
-      float v[E];
-      R.load((int)c, v);
+  auto add = [&](float x, int at) __attribute__((always_inline)) {
+    if (x > -INFINITY && x >= least) {
+      const int p = atomicAdd(&list->n, 1);
+      if (p < TS_LIST) {
+        list->x[p] = x;
+        list->at[p] = at;
+      }
+    }
+  };
+  add(xe, je);
+  if (ONE) {
+    if (mine >= least) {
 #pragma unroll
-      for (int j = 0; j < E; ++j)
-        if (v[j] > -INFINITY && v[j] >= least) {
-          const int p = atomicAdd(&list->n, 1);
-          if (p < TS_LIST) {
-            list->x[p] = v[j];
-            list->at[p] = (int)c * E - R.skew + j;
-          }
+      for (int u = 0; u < TS_BATCH; ++u)
+#pragma unroll
+        for (int j = 0; j < E; ++j) add(x[u][j], R.head + (c0 + tid + T * u) * E + j);
+    }
+  } else {
+    uint64_t todo = __ballot(mine >= least && mine > -INFINITY);
+    while (todo) {                           // the wave reads these threads' pieces together, four threads' at a time
+      int first[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        first[u] = todo ? c0 + wave * 64 + (int)__builtin_ctzll(todo) : c1;
+        todo &= todo - 1;
+      }
+      for (long off = (long)T * lane; first[0] + off < c1; off += (long)T * 64) {
+        float v[4][1][E];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const long c = first[u] + off;
+          R.template load<1>(c < c1 ? (int)c : c0, 0, c1, v[u]);
         }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (first[u] + off < c1) {
+#pragma unroll
+            for (int j = 0; j < E; ++j) add(v[u][0][j], R.head + (int)(first[u] + off) * E + j);
+          }
+      }
     }
   }
   __syncthreads();
@@ -373,14 +463,15 @@ __device__ __forceinline__ int ts_top(const TsRow<D>& R, int c0, int c1, float m
   for (; found < k; ++found) {               // too many equals: one search per place
     float best = -INFINITY;
     int at = 0x7fffffff;
-    for (int c = c0 + tid; c < c1; c += T) {
-      float v[E];
-      R.load(c, v);
+    auto look = [&](float x, int i) __attribute__((always_inline)) {
+      if (x > -INFINITY && ts_before(px, pat, x, i) && ts_before(x, i, best, at)) { best = x; at = i; }
+    };
+    look(xe, je);
+    for (long c = c0 + tid; c < c1; c += T) {
+      float v[1][E];
+      R.template load<1>((int)c, 0, c1, v);
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const int i = c * E - R.skew + j;
-        if (v[j] > -INFINITY && ts_before(px, pat, v[j], i) && ts_before(v[j], i, best, at)) { best = v[j]; at = i; }
-      }
+      for (int j = 0; j < E; ++j) look(v[0][j], R.head + (int)c * E + j);
     }
 #pragma unroll
     for (int w = 32; w > 0; w >>= 1) {
@@ -402,9 +493,8 @@ __device__ __forceinline__ int ts_top(const TsRow<D>& R, int c0, int c1, float m
   return found;
 }
 
-#define TS_BATCH 4              // pieces that a thread requests before it uses the first
-
-template <class D, int T>
+// ONE: a part is at most one batch per thread.
+template <class D, int T, bool ONE>
 __global__ void __launch_bounds__(T) k_scores_row(TsArgs a) {
   constexpr int E = TsRow<D>::E;
   __shared__ TsList list;
@@ -414,7 +504,8 @@ __global__ void __launch_bounds__(T) k_scores_row(TsArgs a) {
   const long row = a.splits == 1 ? blockIdx.x : blockIdx.x / a.splits;
   const int part = a.splits == 1 ? 0 : (int)(blockIdx.x % a.splits);
   const TsRow<D> R(a.x, a.allowed, row, a.row_stride, a.allowed_stride, a.V);
-  const int c0 = part * a.per_part, c1 = part == a.splits - 1 || c0 + a.per_part > R.pieces ? R.pieces : c0 + a.per_part;
+  int c0, c1;
+  ts_part(R.full, a.splits, a.per_part, part, &c0, &c1);
   const float c = a.inv_temp * TS_LOG2E;
   int64_t t = -1;
   float xt = -INFINITY;
@@ -422,18 +513,12 @@ __global__ void __launch_bounds__(T) k_scores_row(TsArgs a) {
     t = a.tok[row];
     xt = ts_token<D>(a, row, t);
   }
-  ts_acc v = {-INFINITY, 0.f, 0.f};
-  for (long i = c0 + tid; i < c1; i += (long)T * TS_BATCH) {
-    float x[TS_BATCH][E];
-#pragma unroll
-    for (int u = 0; u < TS_BATCH; ++u) {
-      if (i + (long)T * u < c1) {
-        R.load((int)(i + T * u), x[u]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < E; ++j) x[u][j] = -INFINITY;
-      }
-    }
+  const int je = part == 0 ? R.edge(tid) : -1;
+  const float xe = R.one(je);
+  ts_acc v = {xe != xe ? -INFINITY : xe, xe == -INFINITY ? 0.f : xe != xe || xe == INFINITY ? NAN : 1.f, 0.f};
+  float x[TS_BATCH][E];
+  auto batch = [&](int i) __attribute__((always_inline)) {
+    R.template load<TS_BATCH>(i, T, c1, x);
     float m = v.m;
 #pragma unroll
     for (int u = 0; u < TS_BATCH; ++u)
@@ -454,6 +539,15 @@ __global__ void __launch_bounds__(T) k_scores_row(TsArgs a) {
         v.s += e;
         v.t = fmaf(e, ts_factor(d), v.t);
       }
+  };
+  if (ONE) {
+#pragma unroll
+    for (int u = 0; u < TS_BATCH; ++u)
+#pragma unroll
+      for (int j = 0; j < E; ++j) x[u][j] = -INFINITY;
+    if (c0 + tid < c1) batch(c0 + tid);
+  } else {
+    for (long i = c0 + tid; i < c1; i += (long)T * TS_BATCH) batch((int)i);
   }
   const float mine = v.m;
   v = ts_join_wave(v, c);
@@ -468,7 +562,7 @@ __global__ void __launch_bounds__(T) k_scores_row(TsArgs a) {
   if (a.splits > 1) {
     TsPart* P = (TsPart*)a.parts + row * a.splits + part;
     int n = 0;
-    if (a.k) n = ts_top<D, T>(R, c0, c1, mine, a.k, &list, wave_bound, [&](int i, float x, int at) {
+    if (a.k) n = ts_top<D, T, ONE>(R, c0, c1, x, xe, je, mine, a.k, &list, wave_bound, [&](int i, float x, int at) {
       P->x[i] = x;
       P->at[i] = at;
     });
@@ -480,7 +574,7 @@ __global__ void __launch_bounds__(T) k_scores_row(TsArgs a) {
   }
   if (tid == 0) ts_finish(a, row, v, ls, t, xt);
   if (a.k == 0) return;
-  const int n = ts_top<D, T>(R, c0, c1, mine, a.k, &list, wave_bound, [&](int i, float x, int at) {
+  const int n = ts_top<D, T, ONE>(R, c0, c1, x, xe, je, mine, a.k, &list, wave_bound, [&](int i, float x, int at) {
     a.top_ids[row * a.k + i] = at;
     a.top_logp[row * a.k + i] = ts_logp(x, v, ls, a.inv_temp);
   });
@@ -491,14 +585,13 @@ __global__ void __launch_bounds__(T) k_scores_row(TsArgs a) {
 }
 
 #define TS_MAX_SPLITS 64
-// The parts of a row, joined: the sums in the order of the parts (every thread the same), the alternatives from the parts'
+// The parts of a row, joined: the sums by a wave (every wave the same), the alternatives from the parts'
 // own k best as in ts_top.
 template <class D>
 __global__ void __launch_bounds__(256) k_scores_join(TsArgs a) {
   constexpr int MOST = TS_MAX_SPLITS * DRK_TOPK_MAX / 256;
   __shared__ float lx[TS_MAX_SPLITS * DRK_TOPK_MAX];
   __shared__ int lat[TS_MAX_SPLITS * DRK_TOPK_MAX];
-  __shared__ ts_acc lv[TS_MAX_SPLITS];
   __shared__ unsigned wave_bound[4];
   __shared__ int kept;
   const long row = blockIdx.x;
@@ -513,7 +606,9 @@ __global__ void __launch_bounds__(256) k_scores_join(TsArgs a) {
     t = a.tok[row];
     xt = ts_token<D>(a, row, t);
   }
-  if (tid < a.splits) lv[tid] = P[tid].v;
+  ts_acc v = {-INFINITY, 0.f, 0.f};
+  if ((tid & 63) < a.splits) v = P[tid & 63].v;
+  v = ts_join_wave(v, c);
   float x[MOST], mine = -INFINITY;
   int at[MOST];
 #pragma unroll
@@ -530,9 +625,6 @@ __global__ void __launch_bounds__(256) k_scores_join(TsArgs a) {
     }
     mine = fmaxf(mine, x[u]);
   }
-  __syncthreads();
-  ts_acc v = lv[0];
-  for (int p = 1; p < a.splits; ++p) v = ts_join(v, lv[p], c);
   const float ls = ts_log_sum(v);
   if (tid == 0) ts_finish(a, row, v, ls, t, xt);
   if (a.k == 0) return;
@@ -561,7 +653,8 @@ __global__ void __launch_bounds__(256) k_scores_join(TsArgs a) {
 }
 
 // One pass: piece in, piece out.  The columns of the one-hot terms are stored once more at the end, by a thread each, from
-// logits that were read before the first store (dlogits may be the logits: a workgroup reads only what it writes itself).
+// logits that were read before the first store (dlogits may be the logits: a workgroup reads only what it writes itself, and
+// what a batch reads in the place of a piece behind the end is its own thread's, not yet stored).
 // ALIKE: a row of dlogits lies on the 16-byte grid as the row of logits does, so that whole pieces are stored.
 template <class D, int T, bool ALIKE>
 __global__ void __launch_bounds__(T) k_scores_row_bwd(TsBwdArgs a) {
@@ -570,36 +663,38 @@ __global__ void __launch_bounds__(T) k_scores_row_bwd(TsBwdArgs a) {
   const long row = a.splits == 1 ? blockIdx.x : blockIdx.x / a.splits;
   const int part = a.splits == 1 ? 0 : (int)(blockIdx.x % a.splits);
   const TsRow<D> R(a.x, a.allowed, row, a.row_stride, a.allowed_stride, a.V);
-  const int c0 = part * a.per_part, c1 = part == a.splits - 1 || c0 + a.per_part > R.pieces ? R.pieces : c0 + a.per_part;
+  int c0, c1;
+  ts_part(R.full, a.splits, a.per_part, part, &c0, &c1);
   typename D::T* dx = (typename D::T*)a.dx + row * a.V;
   const TsRowGrad g = ts_row_grad(a, row);
   int64_t mine = -1;
   float xm = -INFINITY;
   if (tid <= a.k) {
     mine = tid < a.k ? a.top_ids[row * a.k + tid] : g.g1 != 0.f ? g.t : -1;
-    const long piece = mine < 0 || mine >= a.V ? -1 : (mine + R.skew) / E;
-    if (piece >= c0 && piece < c1) xm = D::get(R.x[mine]);
-    else mine = -1;
+    if (mine >= a.V) mine = -1;
+    if (mine < R.head || mine >= R.tail) mine = part == 0 ? mine : -1;
+    else if ((mine - R.head) / E < c0 || (mine - R.head) / E >= c1) mine = -1;
+    if (mine >= 0) xm = D::get(R.x[mine]);
   }
+  const int je = part == 0 ? R.edge(tid) : -1;
+  const float xe = R.one(je);
   if (T > 64) __syncthreads();
+  if (je >= 0) dx[je] = D::put(ts_dense_grad(xe, g, a.inv_temp) * a.inv_temp);
   for (long i = c0 + tid; i < c1; i += (long)T * TS_BATCH) {
     float x[TS_BATCH][E];
-#pragma unroll
-    for (int u = 0; u < TS_BATCH; ++u)
-      if (i + (long)T * u < c1) R.load((int)(i + T * u), x[u]);
+    R.template load<TS_BATCH>((int)i, T, c1, x);
 #pragma unroll
     for (int u = 0; u < TS_BATCH; ++u) {
-      if (i + (long)T * u >= c1) continue;
-      const int c = (int)(i + T * u), j0 = c * E - R.skew;
+      const long at = i + (long)T * u;
       typename TsRow<D>::piece p;
 #pragma unroll
       for (int j = 0; j < E; ++j) p.v[j] = D::put(ts_dense_grad(x[u][j], g, a.inv_temp) * a.inv_temp);
-      if (ALIKE && R.inside(c)) {
-        *(typename TsRow<D>::piece*)(dx + j0) = p;
+      if (at >= c1) continue;
+      if (ALIKE) {
+        *(typename TsRow<D>::piece*)(dx + R.head + at * E) = p;
       } else {
 #pragma unroll
-        for (int j = 0; j < E; ++j)
-          if (j0 + j >= 0 && j0 + j < a.V) dx[j0 + j] = p.v[j];
+        for (int j = 0; j < E; ++j) dx[R.head + at * E + j] = p.v[j];
       }
     }
   }
@@ -614,12 +709,12 @@ static bool ts_shape_ok(long rows, int V, long row_stride, long allowed_stride, 
 }
 static int ts_size(int dtype) { return dtype == DRK_F32 ? 4 : 2; }
 
-// Pieces of 16 bytes per row (one more when the row may start inside one), threads per row, parts per row.  A row of up to
+// Pieces of 16 bytes per row, threads per row, parts per row.  A row of up to
 // 256 pieces is one wave's: its four loads per lane are in flight together.  With fewer rows than `want` workgroups, a row
 // is split as long as a part keeps one piece per thread.
 static void ts_plan(long rows, int V, int size, long want, bool* wave, int* splits, int* per_part) {
   const int e = 16 / size;
-  const long pieces = ((long)V + e - 1) / e + 1;
+  const long pieces = V / e;
   *wave = pieces <= 256;
   long s = 1;
   if (!*wave && rows < want) {
@@ -647,16 +742,17 @@ static int ts_forward(TsArgs a, bool dense, hipStream_t st) {
   if (a.V <= TS_SMALL_V) {
     const bool vec = dense && ((uintptr_t)a.x & 15) == 0 && (!a.allowed_stride || ((uintptr_t)a.allowed & 7) == 0);
     const dim3 grid((unsigned)((a.rows + 63) / 64));
-    if (vec) hipLaunchKernelGGL((k_scores_small<D, true>), grid, dim3(64), 0, st, a);
-    else hipLaunchKernelGGL((k_scores_small<D, false>), grid, dim3(64), 0, st, a);
+    if (vec) hipLaunchKernelGGL((k_scores_small<D, true>), grid, dim3(64), TS_SMALL_LDS(a.V), st, a);
+    else hipLaunchKernelGGL((k_scores_small<D, false>), grid, dim3(64), TS_SMALL_LDS(a.V), st, a);
     DRK_CHECK_LAUNCH();
     return DRK_OK;
   }
   bool wave;
   ts_plan(a.rows, a.V, (int)sizeof(typename D::T), TS_WANT_FWD, &wave, &a.splits, &a.per_part);
   const dim3 grid((unsigned)(a.rows * a.splits));
-  if (wave) hipLaunchKernelGGL((k_scores_row<D, 64>), grid, dim3(64), 0, st, a);
-  else hipLaunchKernelGGL((k_scores_row<D, 256>), grid, dim3(256), 0, st, a);
+  if (wave) hipLaunchKernelGGL((k_scores_row<D, 64, true>), grid, dim3(64), 0, st, a);
+  else if (a.per_part <= 256 * TS_BATCH) hipLaunchKernelGGL((k_scores_row<D, 256, true>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((k_scores_row<D, 256, false>), grid, dim3(256), 0, st, a);
   DRK_CHECK_LAUNCH();
   if (a.splits > 1) {
     hipLaunchKernelGGL(k_scores_join<D>, dim3((unsigned)a.rows), dim3(256), 0, st, a);
@@ -690,8 +786,8 @@ static int ts_backward(TsBwdArgs a, bool dense, hipStream_t st) {
   if (a.V <= TS_SMALL_V) {
     const bool vec = dense && ((uintptr_t)a.x & 15) == 0 && ((uintptr_t)a.dx & 15) == 0 && (!a.allowed_stride || ((uintptr_t)a.allowed & 7) == 0);
     const dim3 grid((unsigned)((a.rows + 63) / 64));
-    if (vec) hipLaunchKernelGGL((k_scores_small_bwd<D, true>), grid, dim3(64), 0, st, a);
-    else hipLaunchKernelGGL((k_scores_small_bwd<D, false>), grid, dim3(64), 0, st, a);
+    if (vec) hipLaunchKernelGGL((k_scores_small_bwd<D, true>), grid, dim3(64), TS_SMALL_LDS(a.V), st, a);
+    else hipLaunchKernelGGL((k_scores_small_bwd<D, false>), grid, dim3(64), TS_SMALL_LDS(a.V), st, a);
     DRK_CHECK_LAUNCH();
     return DRK_OK;
   }

@@ -156,6 +156,25 @@ def test_degenerate_rows(dev, V):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('V', [70, 301, 9001])
+def test_nan_and_infinity_at_the_edges_of_odd_rows(dev, V):
+    """Rows that start off a 16-byte boundary: their first and last elements take a path of their own."""
+    lg = torch.randn(8, V, generator=torch.Generator().manual_seed(V)).to(torch.bfloat16)
+    for r in range(4):
+        lg[r, 0], lg[r + 4, V - 1] = (math.nan, math.inf, -math.inf, 40.0)[r], (math.nan, math.inf, -math.inf, 40.0)[r]
+    tok = torch.full((8,), V // 3)
+    s = ops.token_scores(lg.to(dev), tok.to(dev), topk=3)
+    logp, H, ids, top, _, _ = oracle(lg, tok, None, 1.0, 3)
+    good = [2, 3, 6, 7]
+    close(s.logp[good], logp[good], 'logp')
+    close(s.entropy[good], H[good], 'entropy')
+    assert torch.equal(s.top_ids.cpu()[good], ids[good])
+    assert torch.isnan(s.logp.cpu()[[0, 1, 4, 5]]).all() and torch.isnan(s.entropy.cpu()[[0, 1, 4, 5]]).all()
+    clean = torch.where(torch.isnan(lg), torch.full_like(lg, -math.inf), lg)          # NaN is no alternative, an infinity is the first
+    assert torch.equal(s.top_ids.cpu(), oracle(torch.where(clean == math.inf, torch.full_like(clean, 1e30), clean), tok, None, 1.0, 3)[2])
+
+
+@pytest.mark.gpu
 def test_tokens_outside_and_unscored(dev):
     lg = torch.randn(4, 9, generator=torch.Generator().manual_seed(0)).to(dev)
     allowed = torch.ones(9, dtype=torch.bool, device=dev)
