@@ -247,7 +247,7 @@ struct TsRowGrad {
   float m, ls, gh, H, g1, whole;
   int64_t t;
 };
-__device__ __forceinline__ TsRowGrad ts_row_grad(const TsBwdArgs& a, long row) {
+__device__ __forceinline__ TsRowGrad ts_row_grad(const TsBwdArgs& a, long row) {      // (`whole` without the alternatives)
   TsRowGrad g;
   const float2 st = *(const float2*)(a.stats + 2 * row);
   g.m = st.x;
@@ -255,22 +255,14 @@ __device__ __forceinline__ TsRowGrad ts_row_grad(const TsBwdArgs& a, long row) {
   g.gh = a.g_entropy ? a.g_entropy[row] : 0.f;
   g.H = a.g_entropy ? a.entropy[row] : 0.f;
   g.t = a.tok[row];
-  g.g1 = a.g_logp && g.t >= 0 && g.t < a.V && a.logp[row] != -INFINITY ? a.g_logp[row] : 0.f;
+  const float lp = a.g_logp ? a.logp[row] : -INFINITY, g1 = a.g_logp ? a.g_logp[row] : 0.f;
+  g.g1 = g.t >= 0 && g.t < a.V && lp != -INFINITY ? g1 : 0.f;
   g.whole = g.g1;
-  for (int r = 0; r < a.k; ++r)
-    if (a.top_ids[row * a.k + r] >= 0) g.whole += a.g_top[row * a.k + r];
   return g;
 }
 __device__ __forceinline__ float ts_dense_grad(float x, const TsRowGrad& g, float inv_temp) {
   const float lp = (x - g.m) * inv_temp - g.ls, p = ts_exp2(lp * TS_LOG2E);
   return x == -INFINITY ? 0.f : -p * (g.whole + g.gh * (ts_factor(lp) + g.H));
-}
-// what the one-hot terms add to column j
-__device__ __forceinline__ float ts_hot(const TsBwdArgs& a, long row, const TsRowGrad& g, int64_t j) {
-  float h = j == g.t ? g.g1 : 0.f;
-  for (int r = 0; r < a.k; ++r)
-    if (a.top_ids[row * a.k + r] == j) h += a.g_top[row * a.k + r];
-  return h;
 }
 
 template <class D, bool VEC>
@@ -284,7 +276,13 @@ __global__ void __launch_bounds__(64) k_scores_small_bwd(TsBwdArgs a) {
   ts_stage<D, VEC>((const typename D::T*)a.x + row0 * a.row_stride, own_list ? a.allowed + row0 * V : nullptr, a.row_stride, V, n, lds);
   __syncthreads();
   if (row < a.rows) {
-    const TsRowGrad g = ts_row_grad(a, row);
+    TsRowGrad g = ts_row_grad(a, row);
+#pragma unroll 4
+    for (int r = 0; r < a.k; ++r) {
+      const int64_t j = a.top_ids[row * a.k + r];
+      const float gr = a.g_top[row * a.k + r];
+      g.whole += j >= 0 ? gr : 0.f;
+    }
     for (int j = 0; j < V; j += 8) {
       float x[8];
       ts_eight(lds, base, j, V, on, x);
@@ -666,13 +664,27 @@ __global__ void __launch_bounds__(T) k_scores_row_bwd(TsBwdArgs a) {
   int c0, c1;
   ts_part(R.full, a.splits, a.per_part, part, &c0, &c1);
   typename D::T* dx = (typename D::T*)a.dx + row * a.V;
-  const TsRowGrad g = ts_row_grad(a, row);
-  int64_t mine = -1;
-  float xm = -INFINITY;
-  if (tid <= a.k) {
-    mine = tid < a.k ? a.top_ids[row * a.k + tid] : g.g1 != 0.f ? g.t : -1;
+  TsRowGrad g = ts_row_grad(a, row);
+  // lane r of every wave holds alternative r; the sum runs over the lanes
+  const int lane = tid & 63;
+  int id = -1;
+  float gr = 0.f;
+  if (lane < a.k) {
+    id = (int)a.top_ids[row * a.k + lane];
+    gr = id >= 0 ? a.g_top[row * a.k + lane] : 0.f;
+  }
+  if (a.k) g.whole += ts_wave(gr, [](float u, float v) { return u + v; });
+  // thread r < k stores alternative r's column once more, thread k the given token's: what the one-hot terms add to it
+  int mine = tid < a.k ? id : tid == a.k && g.g1 != 0.f ? (int)g.t : -1;
+  float xm = -INFINITY, hot = mine >= 0 && mine == g.t ? g.g1 : 0.f;
+  for (int r = 0; r < a.k; ++r) {
+    const int other = __builtin_amdgcn_readlane(id, r);
+    const float go = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(gr), r));
+    hot += other == mine ? go : 0.f;
+  }
+  if (mine >= 0) {
     if (mine >= a.V) mine = -1;
-    if (mine < R.head || mine >= R.tail) mine = part == 0 ? mine : -1;
+    else if (mine < R.head || mine >= R.tail) mine = part == 0 ? mine : -1;
     else if ((mine - R.head) / E < c0 || (mine - R.head) / E >= c1) mine = -1;
     if (mine >= 0) xm = D::get(R.x[mine]);
   }
@@ -699,7 +711,7 @@ __global__ void __launch_bounds__(T) k_scores_row_bwd(TsBwdArgs a) {
     }
   }
   __syncthreads();
-  if (mine >= 0) dx[mine] = D::put((ts_dense_grad(xm, g, a.inv_temp) + ts_hot(a, row, g, mine)) * a.inv_temp);
+  if (mine >= 0) dx[mine] = D::put((ts_dense_grad(xm, g, a.inv_temp) + hot) * a.inv_temp);
 }
 
 // ------------------------------------------------------------------------------------------------ C ABI

@@ -618,19 +618,38 @@ _SCORE_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 TokenScores = collections.namedtuple('TokenScores', 'logp entropy top_ids top_logp stats')
 
 
-def _here(name, *tensors):
-    """Every tensor is on the current device: its stream is the one the launch goes to."""
-    for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise _lib.DrakesHipError(f'{name}: expected tensors on the GPU (drakes_amd has no CPU path)')
-        if t.device.index != torch.cuda.current_device():
-            raise ValueError(f'{name}: tensor on {t.device}, but the current device is cuda:{torch.cuda.current_device()}')
+def _at(t, dtype, name, dev):
+    """Address of a contiguous tensor of this type on device `dev`, the current one: its stream is the one that the launch
+    goes to.  (These calls take microseconds on the host: addresses and the stream are passed as plain numbers.)"""
+    if t is None:
+        return None
+    if not t.is_cuda:
+        raise _lib.DrakesHipError(f'{name}: expected a tensor on the GPU (drakes_amd has no CPU path)')
+    if t.dtype is not dtype:
+        raise TypeError(f'{name}: expected {dtype}, got {t.dtype}')
+    if t.get_device() != dev:
+        raise ValueError(f'{name}: tensor on {t.device}, but the current device is cuda:{dev}')
+    if not t.is_contiguous():
+        raise ValueError(f'{name}: tensor must be contiguous')
+    return t.data_ptr()
+
+
+def _current():
+    """(current device, its current stream's handle)"""
+    dev = torch.cuda.current_device()
+    return dev, torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _shaped(t, shape, name):
+    if t is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f'{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}')
+    return t
 
 
 def _row_stride(t, name):
     """Elements between the rows [..., V] of `t`: the last dimension is contiguous and the leading ones step evenly."""
+    if t.is_contiguous():
+        return t.shape[-1]
     if t.shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f'{name}: the last dimension must be contiguous')
     stride, rows = None, 1
@@ -646,25 +665,30 @@ def _row_stride(t, name):
 
 
 def _score_args(name, logits, tokens, allowed, temp):
+    """(device, stream, arguments that the two calls share)"""
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
         raise _lib.DrakesHipError(f'{name}: expected logits on the GPU (drakes_amd has no CPU path)')
-    if logits.dtype not in _SCORE_TYPES:
+    kind = _SCORE_TYPES.get(logits.dtype)
+    if kind is None:
         raise TypeError(f'{name}: logits are float32, bfloat16 or float16, got {logits.dtype}')
-    if logits.ndim < 1 or logits.shape[-1] < 1 or tuple(tokens.shape) != tuple(logits.shape[:-1]):
+    if logits.ndim < 1 or logits.shape[-1] < 1 or tokens.shape != logits.shape[:-1]:
         raise ValueError(f'{name}: logits [..., V] and tokens [...], got {tuple(logits.shape)} and {tuple(tokens.shape)}')
-    if not (0.0 < temp < math.inf):
+    if not 0.0 < temp < math.inf:
         raise ValueError(f'{name}: temp must be positive, got {temp}')
-    V = logits.shape[-1]
+    dev, stream = _current()
+    if logits.get_device() != dev:
+        raise ValueError(f'{name}: logits on {logits.device}, but the current device is cuda:{dev}')
     al, al_stride = None, 0
     if allowed is not None:
-        if allowed.dtype not in (torch.bool, torch.uint8):
+        if allowed.dtype is not torch.bool and allowed.dtype is not torch.uint8:
             raise TypeError(f'{name}: allowed is bool or uint8, got {allowed.dtype}')
-        if tuple(allowed.shape) not in ((V,), tuple(logits.shape)):
+        if allowed.shape != logits.shape[-1:] and allowed.shape != logits.shape:
             raise ValueError(f'{name}: allowed has shape [V] or that of the logits, got {tuple(allowed.shape)}')
-        al, al_stride = _dev_ptr(allowed, allowed.dtype, 'allowed'), V if allowed.ndim > 1 or logits.ndim == 1 else 0
-    _here(name, logits, tokens, allowed)
-    return (ctypes.c_void_p(logits.data_ptr()), _SCORE_TYPES[logits.dtype], _row_stride(logits, name), _i(tokens, 'tokens'), al,
-            al_stride, float(temp))
+        al = _at(allowed, allowed.dtype, 'allowed', dev)
+        if allowed.ndim > 1:
+            al_stride = logits.shape[-1]
+    return dev, stream, (logits.data_ptr(), kind, _row_stride(logits, name), _at(tokens, torch.int64, 'tokens', dev), al, al_stride,
+                         temp)
 
 
 def token_scores(logits, tokens, *, allowed=None, temp=1.0, topk=0, entropy=True):
@@ -672,40 +696,47 @@ def token_scores(logits, tokens, *, allowed=None, temp=1.0, topk=0, entropy=True
 
     logits [..., V] float32 / bfloat16 / float16 (a slice of wider rows will do), tokens int64 [...]: negative = not
     scored; allowed: bool / uint8 [V] or [..., V], the columns that count.  -> TokenScores, float32."""
-    args = _score_args('token_scores', logits, tokens, allowed, temp)
-    V = logits.shape[-1]
+    dev, stream, args = _score_args('token_scores', logits, tokens, allowed, temp)
+    V, shape, on = logits.shape[-1], tokens.shape, logits.device
     if not 0 <= topk <= min(V, TOPK_MAX):
         raise ValueError(f'token_scores: topk must be in [0, min(V, {TOPK_MAX})], got {topk}')
-    new = lambda *last, dtype=torch.float32: torch.empty(*tokens.shape, *last, dtype=dtype, device=logits.device)
-    s = TokenScores(new(), new() if entropy else None, new(topk, dtype=torch.int64) if topk else None,
-                    new(topk) if topk else None, new(2))
+    f32 = torch.float32
+    logp, stats = torch.empty(shape, dtype=f32, device=on), torch.empty((*shape, 2), dtype=f32, device=on)
+    ent = torch.empty(shape, dtype=f32, device=on) if entropy else None
+    ids = torch.empty((*shape, topk), dtype=torch.int64, device=on) if topk else None
+    top = torch.empty((*shape, topk), dtype=f32, device=on) if topk else None
     need = _lib.load().drk_token_scores_workspace_bytes(tokens.numel(), V, args[1])
-    ws = _scratch(need, logits.device) if need else None
-    _lib.call('drk_token_scores', *args, topk, _raw(s.logp), _raw(s.entropy), _raw(s.top_ids), _raw(s.top_logp), _raw(s.stats),
-              tokens.numel(), V, _raw(ws), need, _stream())
-    return s
+    ws = _scratch(need, on) if need else None
+    _lib.call('drk_token_scores', *args, topk, logp.data_ptr(), ent.data_ptr() if entropy else None, ids.data_ptr() if topk else None,
+              top.data_ptr() if topk else None, stats.data_ptr(), tokens.numel(), V, ws.data_ptr() if need else None, need, stream)
+    return TokenScores(logp, ent, ids, top, stats)
 
 
 def token_scores_bwd(logits, tokens, scores, *, g_logp=None, g_entropy=None, g_top=None, allowed=None, temp=1.0, out=None):
     """dlogits (dense, of the logits' type) from the gradients of logp, entropy and top_logp (drk_token_scores_bwd);
     `scores`: what token_scores gave for the same arguments.  out: dense; it may be the logits themselves."""
-    args = _score_args('token_scores_bwd', logits, tokens, allowed, temp)
-    V = logits.shape[-1]
-    shape = tuple(tokens.shape)
+    name, f32 = 'token_scores_bwd', torch.float32
+    dev, stream, args = _score_args(name, logits, tokens, allowed, temp)
+    shape = tokens.shape
     if g_entropy is not None and scores.entropy is None:
         raise ValueError('token_scores_bwd: g_entropy needs the entropy')
     if g_top is not None and scores.top_ids is None:
         raise ValueError('token_scores_bwd: g_top needs the top alternatives')
     k = scores.top_ids.shape[-1] if g_top is not None else 0
-    for t, want, name in ((g_logp, shape, 'g_logp'), (g_entropy, shape, 'g_entropy'), (g_top, shape + (k,), 'g_top'),
-                          (scores.stats, shape + (2,), 'stats'), (scores.logp, shape, 'logp'), (out, tuple(logits.shape), 'out')):
-        if t is not None and tuple(t.shape) != want:
-            raise ValueError(f'token_scores_bwd: {name} has shape {want}, got {tuple(t.shape)}')
-    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if out is None else out
-    _here('token_scores_bwd', g_logp, g_entropy, g_top, *scores, out)
-    _lib.call('drk_token_scores_bwd', *args, k, _f(scores.stats, 'stats'), _f(scores.logp, 'logp'), _f(scores.entropy, 'entropy') if g_entropy is not None else None,
-              _i(scores.top_ids, 'top_ids') if k else None, _f(g_logp, 'g_logp'), _f(g_entropy, 'g_entropy'), _f(g_top, 'g_top'),
-              _dev_ptr(out, logits.dtype, 'out'), tokens.numel(), V, _stream())
+    _shaped(g_logp, shape, name + ': g_logp'), _shaped(g_entropy, shape, name + ': g_entropy')
+    _shaped(scores.logp, shape, name + ': logp'), _shaped(scores.stats, (*shape, 2), name + ': stats')
+    _shaped(out, logits.shape, name + ': out')
+    if k:
+        _shaped(g_top, (*shape, k), name + ': g_top'), _shaped(scores.top_ids, (*shape, k), name + ': top_ids')
+    if g_entropy is not None:
+        _shaped(scores.entropy, shape, name + ': entropy')
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    _lib.call('drk_token_scores_bwd', *args, k, _at(scores.stats, f32, 'stats', dev), _at(scores.logp, f32, 'logp', dev),
+              _at(scores.entropy, f32, 'entropy', dev) if g_entropy is not None else None,
+              _at(scores.top_ids, torch.int64, 'top_ids', dev) if k else None, _at(g_logp, f32, 'g_logp', dev),
+              _at(g_entropy, f32, 'g_entropy', dev), _at(g_top, f32, 'g_top', dev), _at(out, logits.dtype, 'out', dev), tokens.numel(),
+              logits.shape[-1], stream)
     return out
 
 
@@ -718,22 +749,17 @@ Checkpoint8 = collections.namedtuple('Checkpoint8', 'codes exps rstd gates')
 def _rows128(t, name):
     if not isinstance(t, torch.Tensor) or t.ndim != 3 or t.shape[-1] != C:
         raise ValueError(f'{name}: expected a tensor [B, L, {C}]')
+    if not t.is_cuda:
+        raise _lib.DrakesHipError(f'{name}: expected tensors on the GPU (drakes_amd has no CPU path)')
     return t.shape[0], t.shape[1]
 
 
-def _shaped(t, shape, name):
-    if t is not None and tuple(t.shape) != tuple(shape):
-        raise ValueError(f'{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}')
-    return t
-
-
-def _ck8(ck, B, L, name, rstd=False):
-    _shaped(ck.codes, (B, L, C), f'{name}: codes'), _shaped(ck.exps, (B, L, C // 32), f'{name}: exps')
-    _shaped(ck.rstd, (B, L), f'{name}: rstd'), _shaped(ck.gates, (B, L, C // 8), f'{name}: gates')
-    if rstd and ck.rstd is None:
-        raise ValueError(f'{name}: the checkpoint was kept without a LayerNorm (rstd is None)')
-    _here(name, ck.codes, ck.exps, ck.rstd, ck.gates)
-    return _dev_ptr(ck.codes, torch.int8, 'codes'), _dev_ptr(ck.exps, torch.uint8, 'exps')
+def _ck8(ck, B, L, name, dev):
+    """Addresses of a checkpoint's four blocks."""
+    _shaped(ck.codes, (B, L, C), name), _shaped(ck.exps, (B, L, C // 32), name)
+    _shaped(ck.rstd, (B, L), name), _shaped(ck.gates, (B, L, C // 8), name)
+    return (_at(ck.codes, torch.int8, 'codes', dev), _at(ck.exps, torch.uint8, 'exps', dev), _at(ck.rstd, torch.float32, 'rstd', dev),
+            _at(ck.gates, torch.uint8, 'gates', dev))
 
 
 def _scratch(nbytes, device):
@@ -746,29 +772,32 @@ def ln_fwd_ck8(feat, tbias_layer, tb_stride, gamma, beta, *, out=None, relu_mask
     """(h, Checkpoint8) of feat float32 [B,L,128]: h = bf16(LayerNorm(feat + tbias) * gamma + beta) and its normalised input
     kept in 8 bits; gamma None: no LayerNorm, h = bf16(feat) and feat itself is kept.  Gates as bits: from relu_mask uint8
     [B,L,128], or (gate_self) from feat > 0.  tbias_layer, tb_stride: as for ln_fwd_bf16."""
-    B, L = _rows128(feat, 'ln_fwd_ck8')
+    name, f32, u8 = 'ln_fwd_ck8', torch.float32, torch.uint8
+    B, L = _rows128(feat, name)
     if (gamma is None) != (beta is None) or (gamma is None and tbias_layer is not None):
         raise ValueError('ln_fwd_ck8: gamma and beta come together, and tbias needs them')
     if relu_mask is not None and gate_self:
         raise ValueError('ln_fwd_ck8: gates come from relu_mask or from feat, not from both')
     _shaped(relu_mask, (B, L, C), 'ln_fwd_ck8: relu_mask'), _shaped(out, (B, L, C), 'ln_fwd_ck8: out')
     _shaped(gamma, (C,), 'ln_fwd_ck8: gamma'), _shaped(beta, (C,), 'ln_fwd_ck8: beta')
+    dev, stream = _current()
+    tb = None
     if tbias_layer is not None:
-        if tbias_layer.dtype != torch.float32 or not tbias_layer.is_cuda or tbias_layer.stride(-1) != 1:
-            raise ValueError('ln_fwd_ck8: tbias is float32 on the GPU, contiguous over its channels')
+        if tbias_layer.dtype is not f32 or not tbias_layer.is_cuda or tbias_layer.get_device() != dev or tbias_layer.stride(-1) != 1:
+            raise ValueError(f'ln_fwd_ck8: tbias is float32 on cuda:{dev}, contiguous over its channels')
         # the last row read starts (B - 1) * tb_stride elements behind the first
         held = tbias_layer.untyped_storage().nbytes() // 4 - tbias_layer.storage_offset()
         if tb_stride < 0 or max(B - 1, 0) * tb_stride + C > held:
             raise ValueError('ln_fwd_ck8: tbias does not hold a row for every sequence at this tb_stride')
-    _here('ln_fwd_ck8', feat, tbias_layer, gamma, beta, relu_mask, out)
-    new = lambda n, dt: torch.empty(B, L, n, dtype=dt, device=feat.device)
-    out = new(C, torch.bfloat16) if out is None else out
-    ck = Checkpoint8(new(C, torch.int8), new(C // 32, torch.uint8),
-                     torch.empty(B, L, dtype=torch.float32, device=feat.device) if gamma is not None else None,
-                     new(C // 8, torch.uint8) if relu_mask is not None or gate_self else None)
-    _lib.call('drk_ln_fwd_ck8', _f(feat, 'feat'), _raw(tbias_layer), tb_stride, _f(gamma, 'gamma'), _f(beta, 'beta'),
-              _dev_ptr(relu_mask, torch.uint8, 'relu_mask'), int(gate_self), _b16(out, 'h'), _raw(ck.codes), _raw(ck.exps),
-              _raw(ck.rstd), _raw(ck.gates), B, L, int(gamma is not None), _stream())
+        tb = tbias_layer.data_ptr()
+    on, ln, gates = feat.device, gamma is not None, relu_mask is not None or gate_self
+    out = torch.empty((B, L, C), dtype=torch.bfloat16, device=on) if out is None else out
+    ck = Checkpoint8(torch.empty((B, L, C), dtype=torch.int8, device=on), torch.empty((B, L, C // 32), dtype=u8, device=on),
+                     torch.empty((B, L), dtype=f32, device=on) if ln else None,
+                     torch.empty((B, L, C // 8), dtype=u8, device=on) if gates else None)
+    _lib.call('drk_ln_fwd_ck8', _at(feat, f32, 'feat', dev), tb, tb_stride, _at(gamma, f32, 'gamma', dev), _at(beta, f32, 'beta', dev),
+              _at(relu_mask, u8, 'relu_mask', dev), int(gate_self), _at(out, torch.bfloat16, 'out', dev), ck.codes.data_ptr(),
+              ck.exps.data_ptr(), ck.rstd.data_ptr() if ln else None, ck.gates.data_ptr() if gates else None, B, L, int(ln), stream)
     return out, ck
 
 
@@ -776,13 +805,13 @@ def ck8_unpack(ck, dtype=torch.float32, out=None):
     """The values a checkpoint stands for, [B,L,128] float32 or bfloat16 (exact in both)."""
     if out is not None:
         dtype = out.dtype
-    if dtype not in (torch.float32, torch.bfloat16):
+    if dtype is not torch.float32 and dtype is not torch.bfloat16:
         raise TypeError(f'ck8_unpack: float32 or bfloat16, got {dtype}')
     B, L = _rows128(ck.codes, 'ck8_unpack')
-    codes, exps = _ck8(ck, B, L, 'ck8_unpack')
-    out = torch.empty(B, L, C, dtype=dtype, device=ck.codes.device) if out is None else _shaped(out, (B, L, C), 'ck8_unpack: out')
-    _here('ck8_unpack', out)
-    _lib.call('drk_ck8_unpack', codes, exps, _dev_ptr(out, dtype, 'out'), _SCORE_TYPES[dtype], B, L, _stream())
+    dev, stream = _current()
+    codes, exps, _, _ = _ck8(ck, B, L, 'ck8_unpack', dev)
+    out = torch.empty((B, L, C), dtype=dtype, device=ck.codes.device) if out is None else _shaped(out, (B, L, C), 'ck8_unpack: out')
+    _lib.call('drk_ck8_unpack', codes, exps, _at(out, dtype, 'out', dev), _SCORE_TYPES[dtype], B, L, stream)
     return out
 
 
@@ -791,21 +820,24 @@ def ln_bwd_ck8(dh, ck, gamma, g_resid, *, dfeat=None, dxin=None, sums=None, hand
     with hand_over dc = bf16(dfeat * gate), the output gradient of the convolution below.  hand_over False: dc is None and
     dfeat comes gated if the checkpoint has gates.  dfeat may be dh or g_resid; dxin: receives dL/d(LayerNorm input);
     sums float32 [4,128] += (dgamma, dbeta, dtime_bias, column sums of the gated dfeat)."""
-    B, L = _rows128(dh, 'ln_bwd_ck8')
-    codes, exps = _ck8(ck, B, L, 'ln_bwd_ck8', rstd=True)
-    _shaped(gamma, (C,), 'ln_bwd_ck8: gamma'), _shaped(sums, (4, C), 'ln_bwd_ck8: sums')
-    for t, name in ((g_resid, 'g_resid'), (dfeat, 'dfeat'), (dxin, 'dxin')):
-        _shaped(t, (B, L, C), f'ln_bwd_ck8: {name}')
+    name, f32 = 'ln_bwd_ck8', torch.float32
+    B, L = _rows128(dh, name)
+    dev, stream = _current()
+    codes, exps, rstd, gates = _ck8(ck, B, L, name, dev)
+    if rstd is None and B * L:
+        raise ValueError('ln_bwd_ck8: the checkpoint was kept without a LayerNorm (rstd is None)')
     if hand_over and ck.gates is None:
         raise ValueError('ln_bwd_ck8: the checkpoint has no gates to hand over')
-    _here('ln_bwd_ck8', dh, gamma, g_resid, dfeat, dxin, sums)
-    dfeat = torch.empty_like(dh) if dfeat is None else dfeat
-    dc = torch.empty(B, L, C, dtype=torch.bfloat16, device=dh.device) if hand_over else None
+    _shaped(gamma, (C,), 'ln_bwd_ck8: gamma'), _shaped(sums, (4, C), 'ln_bwd_ck8: sums')
+    _shaped(g_resid, (B, L, C), 'ln_bwd_ck8: g_resid'), _shaped(dfeat, (B, L, C), 'ln_bwd_ck8: dfeat')
+    _shaped(dxin, (B, L, C), 'ln_bwd_ck8: dxin')
+    dfeat = torch.empty((B, L, C), dtype=f32, device=dh.device) if dfeat is None else dfeat
+    dc = torch.empty((B, L, C), dtype=torch.bfloat16, device=dh.device) if hand_over else None
     need = _lib.load().drk_ln_bwd_ck8_workspace_bytes(B, L) if sums is not None else 0
     ws = _scratch(need, dh.device) if need else None
-    _lib.call('drk_ln_bwd_ck8', _f(dh, 'dh'), codes, exps, _f(ck.rstd, 'rstd'), _f(gamma, 'gamma'), _f(g_resid, 'g_resid'),
-              _dev_ptr(ck.gates, torch.uint8, 'gates'), _f(dfeat, 'dfeat'), _raw(dc), _f(dxin, 'dxin'), _f(sums, 'sums'), B, L,
-              _raw(ws), need, _stream())
+    _lib.call('drk_ln_bwd_ck8', _at(dh, f32, 'dh', dev), codes, exps, rstd, _at(gamma, f32, 'gamma', dev), _at(g_resid, f32, 'g_resid', dev),
+              gates, _at(dfeat, f32, 'dfeat', dev), dc.data_ptr() if hand_over else None, _at(dxin, f32, 'dxin', dev),
+              _at(sums, f32, 'sums', dev), B, L, ws.data_ptr() if need else None, need, stream)
     return dfeat, dc
 
 
@@ -813,14 +845,15 @@ def gate_ck8(g, gates, *, colsum=None):
     """dc = bf16(g * gate) of g float32 [B,L,128] with a checkpoint's gate bits; colsum [128] += column sums of g * gate."""
     B, L = _rows128(g, 'gate_ck8')
     _shaped(gates, (B, L, C // 8), 'gate_ck8: gates'), _shaped(colsum, (C,), 'gate_ck8: colsum')
-    _here('gate_ck8', g, gates, colsum)
-    dc = torch.empty(B, L, C, dtype=torch.bfloat16, device=g.device)
+    dev, stream = _current()
+    dc = torch.empty((B, L, C), dtype=torch.bfloat16, device=g.device)
     sums = torch.zeros(4, C, dtype=torch.float32, device=g.device) if colsum is not None else None
     need = _lib.load().drk_ln_bwd_ck8_workspace_bytes(B, L) if sums is not None else 0
     ws = _scratch(need, g.device) if need else None
-    _lib.call('drk_ln_bwd_ck8', _f(g, 'g'), None, None, None, None, None, _dev_ptr(gates, torch.uint8, 'gates'), None, _raw(dc),
-              None, _raw(sums), B, L, _raw(ws), need, _stream())
+    _lib.call('drk_ln_bwd_ck8', _at(g, torch.float32, 'g', dev), None, None, None, None, None, _at(gates, torch.uint8, 'gates', dev), None,
+              dc.data_ptr(), None, sums.data_ptr() if need else None, B, L, ws.data_ptr() if need else None, need, stream)
     if colsum is not None:
+        _at(colsum, torch.float32, 'colsum', dev)
         colsum += sums[3]
     return dc
 
@@ -828,17 +861,18 @@ def gate_ck8(g, gates, *, colsum=None):
 def conv_wgrad_ck8(ck, gamma, beta, dc, dwt, dilation):
     """dwt float32 [taps,128(ci),128(co)] += sum_rows h[row + off][ci] * dc[row][co], h = gamma * xq + beta of a checkpoint
     (gamma, beta None: h = xq), dc bf16 [B,L,128]; exact products, fp32 sums in a fixed order."""
-    B, L = _rows128(dc, 'conv_wgrad_ck8')
-    codes, exps = _ck8(ck, B, L, 'conv_wgrad_ck8')
+    name, f32 = 'conv_wgrad_ck8', torch.float32
+    B, L = _rows128(dc, name)
+    dev, stream = _current()
+    codes, exps, _, _ = _ck8(ck, B, L, name, dev)
     if (gamma is None) != (beta is None):
         raise ValueError('conv_wgrad_ck8: gamma and beta come together')
-    _shaped(gamma, (C,), 'conv_wgrad_ck8: gamma'), _shaped(beta, (C,), 'conv_wgrad_ck8: beta')
     taps = dwt.shape[0]
+    _shaped(gamma, (C,), 'conv_wgrad_ck8: gamma'), _shaped(beta, (C,), 'conv_wgrad_ck8: beta')
     _shaped(dwt, (taps, C, C), 'conv_wgrad_ck8: dwt')
     if not (1 <= taps <= 9 and taps % 2 == 1) or dilation < 0:
         raise ValueError(f'conv_wgrad_ck8: an odd number of taps up to 9 and dilation >= 0, got {taps}, {dilation}')
-    _here('conv_wgrad_ck8', gamma, beta, dc, dwt)
     need = _lib.load().drk_conv_wgrad_ck8_workspace_bytes(B, L, taps, dilation)
     ws = _scratch(need, dc.device)
-    _lib.call('drk_conv_wgrad_ck8', codes, exps, _f(gamma, 'gamma'), _f(beta, 'beta'), _b16(dc, 'dc'), _f(dwt, 'dwt'), B, L, taps,
-              dilation, _raw(ws), need, _stream())
+    _lib.call('drk_conv_wgrad_ck8', codes, exps, _at(gamma, f32, 'gamma', dev), _at(beta, f32, 'beta', dev),
+              _at(dc, torch.bfloat16, 'dc', dev), _at(dwt, f32, 'dwt', dev), B, L, taps, dilation, ws.data_ptr(), need, stream)
