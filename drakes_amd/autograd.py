@@ -235,6 +235,7 @@ class GradSink:
         self.stem_db = None
         self.stem_records = []                           # (B, L, dpre [B,L,128], the call's input): the stem's gradients wait too
         self.deferred_stem = False                       # set by grad_chain: a sink that outlives one backward call
+        self.dwt = None                                  # 8-bit checkpoints: the convolutions' gradients, formed call by call
 
     def group(self, key, sigma, temb):
         """The accumulator row of the forwards that ran at this sigma (key: its value as a Python number, known to the
@@ -245,6 +246,11 @@ class GradSink:
             g = (sigma, temb, torch.zeros(self.W, dtype=torch.float32, device=temb.device))
             self.groups[key] = g
         return g[2]
+
+    def conv(self, dev):
+        if self.dwt is None:
+            self.dwt = torch.zeros(9 * self.n + 1, C, C, dtype=torch.float32, device=dev)
+        return self.dwt
 
     def stem(self, dev):
         if self.stem_dw is None:
@@ -261,7 +267,7 @@ class GradSink:
         pk = bb.packed()
         dev = next(iter(self.groups.values()))[2].device
         # ---- convolution weights: one launch per layer and shape over all recorded forwards
-        dwt = torch.zeros(9 * n + 1, C, C, dtype=torch.float32, device=dev)
+        dwt = self.conv(dev)
         by_shape = {}
         for B, L, hs, dcs in self.records:
             by_shape.setdefault((B, L), []).append((hs, dcs))
@@ -311,7 +317,7 @@ class GradSink:
         g['time_embedder.1.weight'], g['time_embedder.1.bias'] = d_lin_w, d_lin_b
         for i in range(n):
             g[f'time_layers.{i}.dense.weight'], g[f'time_layers.{i}.dense.bias'] = d_dense_w[i], d_dense_b[i]
-        self.records, self.groups, self.time, self.stem_dw, self.stem_db = [], {}, {}, None, None
+        self.records, self.groups, self.time, self.stem_dw, self.stem_db, self.dwt = [], {}, {}, None, None, None
         self.stem_records = []
         return g
 
@@ -540,13 +546,137 @@ class _BackboneBf16Fn(torch.autograd.Function):
         return (None, dseq if ctx.needs_input_grad[1] else None, None, None, *grads)
 
 
-def backbone_with_grad(bb, seq, sigma, dtype='fp32', flat=None, sink=None, sigma_key=None):
+class _BackboneCk8Fn(torch.autograd.Function):
+    """_BackboneBf16Fn with its activations kept in 8 bits (ops.ln_fwd_ck8): per row and layer 152 bytes — the normalised
+    LayerNorm input, its rstd and the ReLU gates below it as bits — in the place of the fp32 residual snapshot, the bf16
+    LayerNorm output and the gates (784).  The forward's own arithmetic stays bf16 / fp32 throughout: only the backward's
+    LayerNorm and weight gradients see the rounded values.  One launch per step of a layer; weight gradients are formed by
+    each backward call, so that nothing of it is kept either (a chain's sink collects sums, not operands)."""
+
+    @staticmethod
+    def forward(ctx, bb, seq, sigma, sink, *params):
+        from . import fastpath
+        ctx.sink, ctx.sigma_key = (None, None) if sink is None else sink
+        sink = ctx.sink
+        pk, st = bb.packed(), fastpath._packed(bb)
+        vec, w = st['vecs'].view(-1, C), st['wstream']
+        seq = seq.contiguous()
+        B, L = seq.shape[0], seq.shape[1]
+        n, dev = bb.num_layers, seq.device
+        sigma = sigma.to(torch.float32).contiguous()
+        nb = sigma.shape[0]
+        assert nb in (1, B), 'sigma: one value per row or one shared value'
+        hit = sink.time.get(ctx.sigma_key) if (sink is not None and ctx.sigma_key is not None) else None
+        if hit is not None:
+            sigma, temb, tbias = hit
+        else:
+            temb = ops.time_embed_fwd(sigma, pk['four_W'], pk['temb_w'], pk['temb_b'])
+            tbias = ops.time_bias_fwd(temb, pk['dense_w'], pk['dense_b'])
+            if sink is not None and ctx.sigma_key is not None:
+                sink.time[ctx.sigma_key] = (sigma, temb, tbias)
+        tb_stride = tbias.stride(0) if nb == B and B > 1 else 0
+        assert sink is None or not tb_stride, 'a gradient chain shares one sigma per forward'
+        feat = ops.stem_fwd(seq, pk['stem_w'], pk['stem_b'])
+        mask = torch.empty(B, L, C, dtype=torch.uint8, device=dev)
+        h, ck = ops.ln_fwd_ck8(feat, tbias[0, 0], tb_stride, vec[1], vec[2], gate_self=True)
+        kept = [ck]
+        for i in range(n):
+            ops.layer_bf16(h, w[9 * i:], feat, feat=feat, bias=vec[3 * (i + 1)], taps=9, dilation=bb.dilation(i), relu=True,
+                           relu_mask=mask)
+            if i + 1 < n:
+                h, ck = ops.ln_fwd_ck8(feat, tbias[0, i + 1], tb_stride, vec[3 * (i + 1) + 1], vec[3 * (i + 1) + 2], out=h,
+                                       relu_mask=mask)
+            else:                                   # final_conv.0's input: kept as it is
+                h, ck = ops.ln_fwd_ck8(feat, None, 0, None, None, out=h, relu_mask=mask)
+            kept.append(ck)
+        y = ops.layer_bf16(h, w[9 * n:], feat, bias=vec[3 * n + 1], taps=1, dilation=0, relu=True)      # feat's storage
+        ctx.bb, ctx.pk, ctx.seq, ctx.sigma, ctx.temb, ctx.tb_stride = bb, pk, seq, sigma, temb, tb_stride
+        ctx.kept, ctx.y = kept, y
+        ctx.names = [k for k, _ in bb.named_parameters()]
+        return ops.head_out_fwd(y, pk['head2_w'], pk['head2_b'])
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dlogits):
+        from . import fastpath
+        bb, pk, seq, kept, y = ctx.bb, ctx.pk, ctx.seq, ctx.kept, ctx.y
+        if kept is None:
+            raise RuntimeError('the activations of this forward were freed by an earlier backward pass')
+        B, L = seq.shape[0], seq.shape[1]
+        M, n, dev = B * L, bb.num_layers, dlogits.device
+        wT = fastpath._packed_T(bb)
+        dlogits = dlogits.contiguous()
+        want_w = any(ctx.needs_input_grad[4:])     # a frozen model (the KL reference model) only passes the input gradient on
+        sink = ctx.sink if ctx.sink is not None else (GradSink(bb) if want_w else None)
+        dc = torch.empty(B, L, C, dtype=torch.bfloat16, device=dev)
+        colsum = dwt = sums = rows = None
+        if want_w:
+            dwt = sink.conv(dev)
+            acc = sink.group(ctx.sigma_key, ctx.sigma, ctx.temb)
+            slab = sink.W - sink.head_off
+            sums, colsum = acc[:sink.head_off].view(n + 1, 4, C), acc[:sink.head_off].view(n + 1, 4, C)[n, 3]
+            slabs = (M + 127) // 128
+            part = torch.empty(slabs, slab, dtype=torch.float32, device=dev)
+            ops.head_bwd_bf16(dlogits, y, pk['head2_w'], dc, partials=part, part_stride=slab)
+            ops.slab_reduce(part, slabs, slab, acc[sink.head_off:], slab)
+            ops.conv_wgrad_ck8(kept[n], None, None, dc, dwt[9 * n:], 0)
+            if ctx.tb_stride:
+                rows = torch.zeros(n, B, C, dtype=torch.float32, device=dev)
+        else:
+            ops.head_bwd_bf16(dlogits, y, pk['head2_w'], dc)
+        gr = ops.layer_bf16(dc, wT[9 * n:], y, taps=1, dilation=0, relu=False)          # y's storage: the residual-gradient stream
+        dc = ops.gate_ck8(gr, kept[n].gates, colsum=colsum)
+        dh = torch.empty(B, L, C, dtype=torch.float32, device=dev)
+        dxin = torch.empty_like(dh) if rows is not None else None
+        for i in reversed(range(n)):
+            if want_w:
+                ops.conv_wgrad_ck8(kept[i], pk['ln_g'][i], pk['ln_b'][i], dc, dwt[9 * i:9 * i + 9], bb.dilation(i))
+            ops.layer_bf16(dc, wT[9 * i:], dh, taps=9, dilation=bb.dilation(i), relu=False)
+            gr, dc = ops.ln_bwd_ck8(dh, kept[i], pk['ln_g'][i], gr, dfeat=gr, dxin=dxin, sums=sums[i] if want_w else None,
+                                    hand_over=i > 0)
+            if rows is not None:
+                ops.colsum128(dxin, B, L, rows[i])
+        ctx.kept = ctx.y = None
+        dseq = torch.empty_like(seq) if seq.dtype != torch.int64 and ctx.needs_input_grad[1] else None
+        stem_dw = torch.zeros(9, V, C, dtype=torch.float32, device=dev) if not want_w else sink.stem(dev)[0]
+        if want_w or dseq is not None:
+            ops.stem_bwd(gr, seq, pk['stem_w'], stem_dw, dseq)
+        if want_w:
+            sink.stem(dev)[1][0].add_(sums[0, 3])   # layer 0's gated sums are the stem's bias gradient ...
+            sums[0, 3].zero_()                      # ... of this call: the row is kept for the chain's other calls
+        if ctx.sink is not None or not want_w:
+            return (None, dseq, None, None) + (None,) * len(ctx.needs_input_grad[4:])
+        per_row = None
+        if rows is not None:                        # a time bias per batch row: its gradient goes through the time path row by row
+            sink.groups = {0: (ctx.sigma[:1], ctx.temb[:1], acc)}
+            per_row = {k: torch.zeros_like(p) for k, p in
+                       (('dense_w', pk['dense_w']), ('dense_b', pk['dense_b']), ('temb_w', pk['temb_w']), ('temb_b', pk['temb_b']))}
+            ops.time_bwd(rows.permute(1, 0, 2).contiguous(), ctx.sigma, pk['four_W'], ctx.temb, pk['dense_w'], per_row['dense_w'],
+                         per_row['dense_b'], per_row['temb_w'], per_row['temb_b'], torch.zeros(B, C, dtype=torch.float32, device=dev))
+        g = sink.flush()
+        if per_row is not None:
+            g['time_embedder.1.weight'], g['time_embedder.1.bias'] = per_row['temb_w'], per_row['temb_b']
+            for i in range(n):
+                g[f'time_layers.{i}.dense.weight'], g[f'time_layers.{i}.dense.bias'] = per_row['dense_w'][i], per_row['dense_b'][i]
+        return (None, dseq, None, None, *[g.get(k) if ctx.needs_input_grad[4 + j] else None for j, k in enumerate(ctx.names)])
+
+
+def backbone_with_grad(bb, seq, sigma, dtype='fp32', flat=None, sink=None, sigma_key=None, keep=None):
     """dtype 'bf16': the bf16-MFMA layer kernels (gradients within the bf16 bar); 'fp32': the exact-fp32 kernels;
     'bf16x3': those with the convolutions (forward and input gradient) at fp32 grade on the bf16 matrix cores.
     flat: flat_params(bb), built once by a caller that runs many forwards per backward pass (see there); on the bf16 path
-    (sink, flat) = grad_chain(bb) instead, and sigma_key = sigma's value as a Python number when the caller knows it."""
+    (sink, flat) = grad_chain(bb) instead, and sigma_key = sigma's value as a Python number when the caller knows it.
+    keep 'int8' (bf16 path): the activations that the backward reads are kept in 8 bits (_BackboneCk8Fn)."""
     if dtype is True:
         dtype = 'bf16'
+    if keep not in (None, 'int8'):
+        raise ValueError(f"keep: None or 'int8', got {keep!r}")
+    if keep == 'int8':
+        if dtype != 'bf16':
+            raise NotImplementedError(f"activations in 8 bits belong to the bf16 differentiable path (got {dtype!r})")
+        if sink is not None:
+            return _BackboneCk8Fn.apply(bb, seq, sigma, (sink, sigma_key), flat)
+        return _BackboneCk8Fn.apply(bb, seq, sigma, None, *bb.parameters())
     if dtype == 'bf16':      # sink, flat = grad_chain(bb): parameter gradients deferred to the end of the chain
         if sink is not None:
             return _BackboneBf16Fn.apply(bb, seq, sigma, (sink, sigma_key), flat)

@@ -16,7 +16,8 @@ Differences a caller can see, all additive:
     the convolutions at fp32 grade on the bf16 matrix cores (three bf16 planes per operand: logits within ~1e-5 of the
     exact path's, ~3x its speed; under autograd the forward and input-gradient convolutions use it, weight gradients stay
     on the f32 MFMA), or the bf16-MFMA fast path (one launch per `_sample`; differentiable steps on the bf16 layer kernels);
-    `hip_graph = True` replays the fp32 step loop from a captured hipGraph.
+    `hip_checkpoint = 'int8'` keeps the bf16 differentiable path's activations in 8 bits (a quarter of the memory, and
+    gradients within about a percent); `hip_graph = True` replays the fp32 step loop from a captured hipGraph.
 """
 import torch
 import torch.nn as nn
@@ -49,6 +50,7 @@ class Diffusion(nn.Module):
         self.neg_infinity = -1000000.0
         self.hip_dtype = 'fp32'
         self.hip_soft_dtype = None      # differentiable (Gumbel-softmax) steps: None = follow hip_dtype; 'fp32' | 'bf16'
+        self.hip_checkpoint = None      # 'int8': the bf16 differentiable path keeps its activations in 8 bits
         self.hip_graph = False          # fp32 path: replay the step loop from a captured hipGraph (see _sample_graph)
         self._graph = None
         self._validate_configuration()
@@ -102,7 +104,7 @@ class Diffusion(nn.Module):
         sigma = self._process_sigma(sigma)                 # every row holds this one value (known without a device read)
         if not self.time_conditioning or uniform is not None:
             sigma = sigma[:1]                              # one time bias for the batch: same values, one row of work
-        self.backbone.train_dtype = self._soft_dtype()
+        self.backbone.train_dtype, self.backbone.train_keep = self._soft_dtype(), self.hip_checkpoint
         logits = self.backbone(x, sigma)
         return self._subs_parameterization(logits=logits, xt=x)
 
@@ -295,7 +297,7 @@ class Diffusion(nn.Module):
         sigma = self._process_sigma(sigma)
         if not self.time_conditioning:
             sigma = sigma[:1]
-        self.backbone.train_dtype = self._soft_dtype()
+        self.backbone.train_dtype, self.backbone.train_keep = self._soft_dtype(), self.hip_checkpoint
         logits = self.backbone(x, sigma)
         answers = getattr(self, '_answers', None)
         if answers is None or answers.device != logits.device:

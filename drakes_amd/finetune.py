@@ -36,8 +36,8 @@ def ddpm_update_finetune_gradient(model, x, t, dt, copy_flag_temp, return_proces
         sig = sig[:1]                                  # one shared value (all rows are equal)
     if seed is None and uniforms is None:
         seed = model._draw_seed()
-    model.backbone.train_dtype = model._soft_dtype()
-    logits = autograd.backbone_with_grad(model.backbone, x, sig, model._soft_dtype())
+    model.backbone.train_dtype, model.backbone.train_keep = model._soft_dtype(), model.hip_checkpoint
+    logits = autograd.backbone_with_grad(model.backbone, x, sig, model._soft_dtype(), keep=model.hip_checkpoint)
     x_next, flag = autograd.soft_step_with_grad(logits, x, float(mct[0]), float(mcs[0]),
                                                 float(model.config.finetuning.gumbel_softmax_temp), copy_flag_temp,
                                                 seed or 0, step, sample_offset, uniforms, mc_rows)
@@ -62,7 +62,7 @@ def sample_finetune_gradient(model, num_steps=None, eps=1e-5, eval_sp_size=None,
     table = table.tolist()
     bb = model.backbone
     soft_bf16 = model._soft_dtype() == 'bf16'
-    bb.train_dtype = model._soft_dtype()       # Diffusion.forward (the KL term of the fine-tune loop) follows it
+    bb.train_dtype, bb.train_keep = model._soft_dtype(), model.hip_checkpoint      # Diffusion.forward (the KL term of the fine-tune loop) follows them
     x = torch.full((batch, L), model.mask_index, dtype=torch.int64, device=dev)      # _sample_prior, on the device
     last_x_list, condt_list, move_chance_t_list, copy_flag_list = [], [], [], []
     # raw logits (with their graph) of every soft step, keyed by the identity of the state they were computed from: the
@@ -125,7 +125,8 @@ def sample_finetune_gradient(model, num_steps=None, eps=1e-5, eval_sp_size=None,
             grad_on = torch.is_grad_enabled()
             logits = autograd.backbone_with_grad(bb, x, sig, bb.train_dtype, flat=flat if grad_on else None,
                                                  sink=sink if grad_on else None,
-                                                 sigma_key=float(sigma_t) if model.time_conditioning else 0.0)
+                                                 sigma_key=float(sigma_t) if model.time_conditioning else 0.0,
+                                                 keep=model.hip_checkpoint)
             last_x = x
             model._soft_logits_cache[id(x)] = (x, logits, bb._weights_key())
             x, copy_flag = autograd.soft_step_with_grad(logits, x, mc_t, mc_s, temp, copy_flag_temp, seed, i,

@@ -245,7 +245,8 @@ class CNNModel(nn.Module):
             seq = seq.long()
         if torch.is_grad_enabled() and (seq.requires_grad or any(p.requires_grad for p in self.parameters())):
             from ..autograd import backbone_with_grad
-            return backbone_with_grad(self, seq.contiguous(), t.to(torch.float32), getattr(self, 'train_dtype', 'fp32'))
+            return backbone_with_grad(self, seq.contiguous(), t.to(torch.float32), getattr(self, 'train_dtype', 'fp32'),
+                                      keep=getattr(self, 'train_keep', None))
         tbias = self.time_bias(t.to(torch.float32))
         if t.shape[0] not in (1, seq.shape[0]):
             raise ValueError(f't: one value per batch row or one shared value (got {t.shape[0]} for batch {seq.shape[0]})')
