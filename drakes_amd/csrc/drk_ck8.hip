@@ -18,6 +18,7 @@
 #include "../../include/drakes_hip.h"
 
 typedef __bf16 bf16v8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16v4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
@@ -182,14 +183,35 @@ __global__ void __launch_bounds__(256) k_ln_fwd_ck8(CkFwdArgs a) {
   }
 }
 
+// Four channels per thread, four groups in flight: a wave's store is 1 KB (bf16: 512 bytes) in one piece.
 template <bool BF16>
-__global__ void __launch_bounds__(256) k_ck8_unpack(const uint64_t* __restrict__ codes, const unsigned char* __restrict__ exps,
+__global__ void __launch_bounds__(256) k_ck8_unpack(const unsigned* __restrict__ codes, const unsigned char* __restrict__ exps,
                                                     char* __restrict__ out, long n) {
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {     // eight channels each
-    float v[8];
-    decode8(codes[i], exps[i >> 2], v);
-    if (BF16) store8_bf16(out + 16 * i, v);
-    else store8((float*)(out + 32 * i), v);
+  const long step = (long)gridDim.x * 256;
+  for (long i0 = (long)blockIdx.x * 256 + threadIdx.x; i0 < n; i0 += 4 * step) {
+    unsigned q[4], e[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const long i = i0 + u * step < n ? i0 + u * step : i0;
+      q[u] = codes[i];
+      e[u] = exps[i >> 3];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const long i = i0 + u * step;
+      float v[8];
+      decode8(q[u], e[u], v);
+      if (i < n) {
+        if (BF16) {
+          bf16v4 o;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[j] = (__bf16)v[j];
+          *(bf16v4*)(out + 8 * i) = o;
+        } else {
+          *(f32x4*)(out + 16 * i) = f32x4{v[0], v[1], v[2], v[3]};
+        }
+      }
+    }
   }
 }
 
@@ -585,9 +607,18 @@ __global__ void __launch_bounds__(512) k_wgrad_ck8_ring(CwArgs a) {
     u32x4 v = {ones, ones, ones, ones};
     if (!(lb + 31 < L && lb + o_first >= 0 && lb + 31 + o_last < L)) {
       const unsigned mine = cw_inside(lb, L, my_shift);    // lane t finds tap t's rows
+      unsigned rows[CW_NT];
 #pragma unroll
-      for (int i = 0; i < CW_NT; ++i) f.a[i] = cw_clear(f.a[i], mask(__builtin_amdgcn_readlane(mine, i < 4 ? 2 * i + tg : 8)));
-      v &= mask(mine);
+      for (int i = 0; i < CW_NT; ++i) rows[i] = __builtin_amdgcn_readlane(mine, i < 4 ? 2 * i + tg : 8);
+      if (__ballot(mine != 0u && mine != ~0u)) {
+#pragma unroll
+        for (int i = 0; i < CW_NT; ++i) f.a[i] = cw_clear(f.a[i], mask(rows[i]));
+        v &= mask(mine);
+      } else {                                             // every tap all or nothing, as where shifts and lengths are multiples of 32
+#pragma unroll
+        for (int i = 0; i < CW_NT; ++i) f.a[i] = cw_clear(f.a[i], u32x4{rows[i], rows[i], rows[i], rows[i]});
+        v &= mine;
+      }
     }
     load(next, T, buf, ks);
 #pragma unroll
@@ -731,11 +762,11 @@ extern "C" int drk_ln_fwd_ck8(const float* feat, const float* tbias, long tb_str
 extern "C" int drk_ck8_unpack(const signed char* codes, const unsigned char* exps, void* out, int dtype, int B, int L, void* stream) {
   DRK_SHAPE_GUARD("drk_ck8_unpack");
   CKCHECK(codes && exps && out && aligned16(out) && ((uintptr_t)codes & 7) == 0, "drk_ck8_unpack");
-  const long n = (long)B * L * (DRK_C / 8);
-  long grid = (n + 255) / 256;
+  const long n = (long)B * L * (DRK_C / 4);
+  long grid = (n + 1023) / 1024;
   if (grid > CK_FWD_WGS) grid = CK_FWD_WGS;
-  if (dtype == DRK_F32) hipLaunchKernelGGL(k_ck8_unpack<false>, dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, (const uint64_t*)codes, exps, (char*)out, n);
-  else if (dtype == DRK_BF16) hipLaunchKernelGGL(k_ck8_unpack<true>, dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, (const uint64_t*)codes, exps, (char*)out, n);
+  if (dtype == DRK_F32) hipLaunchKernelGGL(k_ck8_unpack<false>, dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, (const unsigned*)codes, exps, (char*)out, n);
+  else if (dtype == DRK_BF16) hipLaunchKernelGGL(k_ck8_unpack<true>, dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, (const unsigned*)codes, exps, (char*)out, n);
   else return drk_set_error_msg(DRK_EINVAL, "drk_ck8_unpack: dtype is DRK_F32 or DRK_BF16");
   DRK_CHECK_LAUNCH();
   return DRK_OK;

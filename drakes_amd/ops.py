@@ -641,7 +641,7 @@ def _current():
 
 
 def _shaped(t, shape, name):
-    if t is not None and tuple(t.shape) != tuple(shape):
+    if t is not None and t.shape != shape:
         raise ValueError(f'{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}')
     return t
 
