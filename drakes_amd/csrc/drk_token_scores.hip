@@ -136,7 +136,7 @@ __device__ __forceinline__ int ts_pad(int i) { return i + (i >> 6); }
 // n consecutive rows -> LDS as floats, -inf in columns that a per-row list leaves out.  VEC: the rows are dense and 16-byte
 // aligned (and so is the list, by its own width): whole 16-byte pieces.
 template <class D, bool VEC>
-__device__ __forceinline__ void ts_stage(const typename D::T* x, const unsigned char* al, long row_stride, int V, int n, float* lds) {
+__device__ __forceinline__ void ts_stage(const typename D::T* x, const unsigned char* al, long row_stride, long al_stride, int V, int n, float* lds) {
   constexpr int E = 16 / sizeof(typename D::T);
   const int lane = threadIdx.x, total = n * V;
   if (VEC) {
@@ -166,7 +166,7 @@ __device__ __forceinline__ void ts_stage(const typename D::T* x, const unsigned 
     const float inv = 1.f / (float)V;
     for (int i = lane; i < total; i += 64) {
       const int r = (int)(((float)i + 0.5f) * inv), c = i - r * V;      // i < 4096: the quotient is exact
-      lds[ts_pad(i)] = al && !al[(long)r * V + c] ? -INFINITY : D::get(x[r * row_stride + c]);
+      lds[ts_pad(i)] = al && !al[r * al_stride + c] ? -INFINITY : D::get(x[r * row_stride + c]);
     }
   }
 }
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(64) k_scores_small(TsArgs a) {
   const bool own_list = a.allowed && a.allowed_stride;
   const uint64_t on = ts_shared_list(own_list ? nullptr : a.allowed, V);
   const int64_t t = row < a.rows ? a.tok[row] : -1;
-  ts_stage<D, VEC>((const typename D::T*)a.x + row0 * a.row_stride, own_list ? a.allowed + row0 * V : nullptr, a.row_stride, V, n, lds);
+  ts_stage<D, VEC>((const typename D::T*)a.x + row0 * a.row_stride, own_list ? a.allowed + row0 * a.allowed_stride : nullptr, a.row_stride, a.allowed_stride, V, n, lds);
   __syncthreads();
   if (row >= a.rows) return;
   const float c = a.inv_temp * TS_LOG2E;
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(64) k_scores_small_bwd(TsBwdArgs a) {
   const int n = (int)(a.rows - row0 < 64 ? a.rows - row0 : 64), V = a.V, base = threadIdx.x * V;
   const bool own_list = a.allowed && a.allowed_stride;
   const uint64_t on = ts_shared_list(own_list ? nullptr : a.allowed, V);
-  ts_stage<D, VEC>((const typename D::T*)a.x + row0 * a.row_stride, own_list ? a.allowed + row0 * V : nullptr, a.row_stride, V, n, lds);
+  ts_stage<D, VEC>((const typename D::T*)a.x + row0 * a.row_stride, own_list ? a.allowed + row0 * a.allowed_stride : nullptr, a.row_stride, a.allowed_stride, V, n, lds);
   __syncthreads();
   if (row < a.rows) {
     TsRowGrad g = ts_row_grad(a, row);

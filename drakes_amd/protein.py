@@ -68,6 +68,8 @@ class Interpolant:
         Positions outside `mask` and negative targets are not scored; the mask token is no answer; allowed: bool [22] or
         [B, L, 22], what else may stand there.  -> (logp, entropy, top_ids, top_logp), differentiable in the model."""
         logits = model(X, aatypes, mask, chain_M, residue_idx, chain_encoding_all)
+        if logits.stride(-1) != 1:
+            logits = logits.contiguous()
         answers = torch.arange(self.num_tokens, device=logits.device) != MASK_TOKEN_INDEX
         if allowed is not None:
             answers = (answers & allowed).contiguous()

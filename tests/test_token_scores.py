@@ -262,6 +262,67 @@ def test_rows_beyond_32_bit_offsets(dev):
     assert float(d[-1, V - 1]) == pytest.approx(1.0, abs=1e-2) and float(d[5, 0]) == pytest.approx(1.0, abs=1e-2)
 
 
+@pytest.mark.gpu
+def test_wider_lists_through_the_c_abi(dev):
+    """A per-row list whose rows are longer than V."""
+    import ctypes
+    from drakes_amd import _lib
+    for V, wide in ((7, 12), (50, 64), (200, 333)):
+        lg = torch.randn(70, V, generator=torch.Generator().manual_seed(V)).to(dev)
+        tok = torch.zeros(70, dtype=torch.int64, device=dev)
+        big = torch.zeros(70, wide, dtype=torch.uint8)
+        big[:, :V] = torch.rand(70, V, generator=torch.Generator().manual_seed(1)) < 0.5
+        ref = ops.token_scores(lg, tok, allowed=big[:, :V].contiguous().to(dev))
+        wide_list = big.to(dev)
+        logp, stats = torch.empty(70, device=dev), torch.empty(70, 2, device=dev)
+        P = lambda t: ctypes.c_void_p(t.data_ptr())
+        _lib.call('drk_token_scores', P(lg), 0, V, P(tok), P(wide_list), wide, 1.0, 0, P(logp), None, None, None, P(stats), 70, V, None, 0,
+                  ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+        assert torch.equal(logp, ref.logp) and torch.equal(stats, ref.stats)
+
+
+@pytest.mark.gpu
+def test_one_row_without_batch_dimensions(dev):
+    lg = torch.randn(30, generator=torch.Generator().manual_seed(1)).to(dev)
+    allowed = torch.arange(30, device=dev) != 4
+    s = ops.token_scores(lg, torch.tensor(7, device=dev), allowed=allowed, topk=2)
+    logp, H, ids, top, _, _ = oracle(lg.unsqueeze(0), torch.tensor([7]), allowed, 1.0, 2)
+    assert s.logp.shape == () and s.top_ids.shape == (2,)
+    close(s.logp.unsqueeze(0), logp, 'logp')
+    assert torch.equal(s.top_ids.cpu(), ids[0])
+
+
+@pytest.mark.gpu
+def test_calls_at_once_on_two_streams(dev):
+    """Split rows and whole ones, forward and backward, on two streams without an order between them."""
+    a, ta, _ = case(70000, (4,), torch.float32, 1, 'none', dev)
+    b, tb, _ = case(70000, (4,), torch.float32, 2, 'none', dev)
+    g = torch.ones(4, device=dev)
+    run = lambda x, t: (lambda s: [*s, ops.token_scores_bwd(x, t, s, g_logp=g)])(ops.token_scores(x, t, topk=7))
+    wa, wb = run(a, ta), run(b, tb)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        for s in (s1, s2):
+            s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s1):
+            ra = run(a, ta)
+        with torch.cuda.stream(s2):
+            rb = run(b, tb)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(ra, wa)) and all(torch.equal(x, y) for x, y in zip(rb, wb))
+
+
+@pytest.mark.gpu
+def test_another_device_is_refused(dev, monkeypatch):
+    lg, tok = torch.zeros(2, 5, device=dev), torch.zeros(2, dtype=torch.int64, device=dev)
+    z = torch.zeros(1, 4, 128, device=dev)
+    monkeypatch.setattr(ops, '_current', lambda: (1, 0))          # as if another GPU were the current one; nothing is launched
+    with pytest.raises(ValueError, match='current device'):
+        ops.token_scores(lg, tok)
+    with pytest.raises(ValueError, match='current device'):
+        ops.ln_fwd_ck8(z, None, 0, None, None)
+
+
 def test_refusals_cpu():
     lg, tok = torch.zeros(2, 5), torch.zeros(2, dtype=torch.int64)
     with pytest.raises(DrakesHipError):
