@@ -299,10 +299,7 @@ class Diffusion(nn.Module):
             sigma = sigma[:1]
         self.backbone.train_dtype, self.backbone.train_keep = self._soft_dtype(), self.hip_checkpoint
         logits = self.backbone(x, sigma)
-        answers = getattr(self, '_answers', None)
-        if answers is None or answers.device != logits.device:
-            answers = torch.arange(self.vocab_size, device=logits.device) != self.mask_index
-            self._answers = answers
+        answers = torch.arange(self.vocab_size, device=logits.device) != self.mask_index
         return token_scores_with_grad(logits, targets.contiguous(), allowed=answers, temp=temp, topk=topk)
 
     # ------------------------------------------------------------------ fine-tuning sampler
