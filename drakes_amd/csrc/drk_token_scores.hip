@@ -99,7 +99,7 @@ struct TsArgs {
   const void* x;
   const int64_t* tok;
   const unsigned char* allowed;
-  long allowed_stride, row_stride, rows;
+  long allowed_stride, row_stride, rows, row0;
   float *logp, *entropy, *stats, *top_logp;
   int64_t* top_ids;
   void* parts;                 // split rows: [rows][splits] TsPart
@@ -237,7 +237,7 @@ struct TsBwdArgs {
   const void* x;
   const int64_t* tok;
   const unsigned char* allowed;
-  long allowed_stride, row_stride, rows;
+  long allowed_stride, row_stride, rows, row0;
   const float *stats, *logp, *entropy, *g_logp, *g_entropy, *g_top;
   const int64_t* top_ids;
   void* dx;
@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(T) k_scores_row(TsArgs a) {
   __shared__ ts_acc wave_acc[T / 64];
   __shared__ unsigned wave_bound[T / 64];
   const int tid = threadIdx.x;
-  const long row = a.splits == 1 ? blockIdx.x : blockIdx.x / a.splits;
+  const long row = a.row0 + (a.splits == 1 ? blockIdx.x : blockIdx.x / a.splits);
   const int part = a.splits == 1 ? 0 : (int)(blockIdx.x % a.splits);
   const TsRow<D> R(a.x, a.allowed, row, a.row_stride, a.allowed_stride, a.V);
   int c0, c1;
@@ -661,7 +661,7 @@ template <class D, int T, bool ALIKE>
 __global__ void __launch_bounds__(T) k_scores_row_bwd(TsBwdArgs a) {
   constexpr int E = TsRow<D>::E;
   const int tid = threadIdx.x;
-  const long row = a.splits == 1 ? blockIdx.x : blockIdx.x / a.splits;
+  const long row = a.row0 + (a.splits == 1 ? blockIdx.x : blockIdx.x / a.splits);
   const int part = a.splits == 1 ? 0 : (int)(blockIdx.x % a.splits);
   const TsRow<D> R(a.x, a.allowed, row, a.row_stride, a.allowed_stride, a.V);
   int c0, c1;
@@ -743,6 +743,11 @@ static void ts_plan(long rows, int V, int size, long want, bool* wave, int* spli
   *splits = (int)((pieces + per - 1) / per);
 }
 #define TS_WANT_FWD 512
+// A launch holds fewer than 2^32 threads: 256 per row make that 2^24 rows (which are never split).
+#define TS_LAUNCH_ROWS ((1L << 24) - 1)
+static unsigned ts_grid(long rows, long row0, int splits) {
+  return (unsigned)((rows - row0 < TS_LAUNCH_ROWS ? rows - row0 : TS_LAUNCH_ROWS) * splits);
+}
 
 extern "C" long drk_token_scores_workspace_bytes(long rows, int V, int dtype) {
   if (rows <= 0 || V <= TS_SMALL_V) return 0;
@@ -764,11 +769,13 @@ static int ts_forward(TsArgs a, bool dense, hipStream_t st) {
   }
   bool wave;
   ts_plan(a.rows, a.V, (int)sizeof(typename D::T), TS_WANT_FWD, &wave, &a.splits, &a.per_part);
-  const dim3 grid((unsigned)(a.rows * a.splits));
-  if (wave) hipLaunchKernelGGL((k_scores_row<D, 64, true>), grid, dim3(64), 0, st, a);
-  else if (a.per_part <= 256 * TS_BATCH) hipLaunchKernelGGL((k_scores_row<D, 256, true>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((k_scores_row<D, 256, false>), grid, dim3(256), 0, st, a);
-  DRK_CHECK_LAUNCH();
+  for (a.row0 = 0; a.row0 < a.rows; a.row0 += TS_LAUNCH_ROWS) {
+    const dim3 grid(ts_grid(a.rows, a.row0, a.splits));
+    if (wave) hipLaunchKernelGGL((k_scores_row<D, 64, true>), grid, dim3(64), 0, st, a);
+    else if (a.per_part <= 256 * TS_BATCH) hipLaunchKernelGGL((k_scores_row<D, 256, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_scores_row<D, 256, false>), grid, dim3(256), 0, st, a);
+    DRK_CHECK_LAUNCH();
+  }
   if (a.splits > 1) {
     hipLaunchKernelGGL(k_scores_join<D>, dim3((unsigned)a.rows), dim3(256), 0, st, a);
     DRK_CHECK_LAUNCH();
@@ -786,7 +793,7 @@ extern "C" int drk_token_scores(const void* logits, int dtype, long row_stride, 
   const long need = drk_token_scores_workspace_bytes(rows, V, dtype);
   TSCHECK(need == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need),
           "drk_token_scores (workspace: 16-byte aligned, drk_token_scores_workspace_bytes(rows, V, dtype) bytes)");
-  const TsArgs a = {logits, tokens, allowed, allowed_stride, row_stride, rows, logp, entropy, stats, top_logp, top_ids, workspace, V, k, 1, 0, 1.f / temp};
+  const TsArgs a = {logits, tokens, allowed, allowed_stride, row_stride, rows, 0, logp, entropy, stats, top_logp, top_ids, workspace, V, k, 1, 0, 1.f / temp};
   const bool dense = row_stride == V && (allowed_stride == 0 || allowed_stride == V);
   if (dtype == DRK_F32) return ts_forward<ts_f32>(a, dense, (hipStream_t)stream);
   if (dtype == DRK_BF16) return ts_forward<ts_bf16>(a, dense, (hipStream_t)stream);
@@ -809,12 +816,14 @@ static int ts_backward(TsBwdArgs a, bool dense, hipStream_t st) {
   bool wave;
   ts_plan(a.rows, a.V, size, TS_WANT_BWD, &wave, &a.splits, &a.per_part);
   const bool alike = (a.row_stride - a.V) * size % 16 == 0 && (((uintptr_t)a.x ^ (uintptr_t)a.dx) & 15) == 0;
-  const dim3 grid((unsigned)(a.rows * a.splits));
-  if (wave && alike) hipLaunchKernelGGL((k_scores_row_bwd<D, 64, true>), grid, dim3(64), 0, st, a);
-  else if (wave) hipLaunchKernelGGL((k_scores_row_bwd<D, 64, false>), grid, dim3(64), 0, st, a);
-  else if (alike) hipLaunchKernelGGL((k_scores_row_bwd<D, 256, true>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((k_scores_row_bwd<D, 256, false>), grid, dim3(256), 0, st, a);
-  DRK_CHECK_LAUNCH();
+  for (a.row0 = 0; a.row0 < a.rows; a.row0 += TS_LAUNCH_ROWS) {
+    const dim3 grid(ts_grid(a.rows, a.row0, a.splits));
+    if (wave && alike) hipLaunchKernelGGL((k_scores_row_bwd<D, 64, true>), grid, dim3(64), 0, st, a);
+    else if (wave) hipLaunchKernelGGL((k_scores_row_bwd<D, 64, false>), grid, dim3(64), 0, st, a);
+    else if (alike) hipLaunchKernelGGL((k_scores_row_bwd<D, 256, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_scores_row_bwd<D, 256, false>), grid, dim3(256), 0, st, a);
+    DRK_CHECK_LAUNCH();
+  }
   return DRK_OK;
 }
 
@@ -828,7 +837,7 @@ extern "C" int drk_token_scores_bwd(const void* logits, int dtype, long row_stri
           "drk_token_scores_bwd");
   TSCHECK(((uintptr_t)stats & 7) == 0, "drk_token_scores_bwd (stats: 8-byte aligned)");
   TSCHECK(dlogits != logits || row_stride == V, "drk_token_scores_bwd (in place: dense rows)");
-  const TsBwdArgs a = {logits, tokens, allowed, allowed_stride, row_stride, rows, stats, logp, entropy, g_logp, g_entropy, g_top, top_ids, dlogits, V, k, 1, 0, 1.f / temp};
+  const TsBwdArgs a = {logits, tokens, allowed, allowed_stride, row_stride, rows, 0, stats, logp, entropy, g_logp, g_entropy, g_top, top_ids, dlogits, V, k, 1, 0, 1.f / temp};
   const bool dense = row_stride == V && (allowed_stride == 0 || allowed_stride == V);
   if (dtype == DRK_F32) return ts_backward<ts_f32>(a, dense, (hipStream_t)stream);
   if (dtype == DRK_BF16) return ts_backward<ts_bf16>(a, dense, (hipStream_t)stream);

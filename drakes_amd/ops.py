@@ -870,8 +870,8 @@ def conv_wgrad_ck8(ck, gamma, beta, dc, dwt, dilation):
     taps = dwt.shape[0]
     _shaped(gamma, (C,), 'conv_wgrad_ck8: gamma'), _shaped(beta, (C,), 'conv_wgrad_ck8: beta')
     _shaped(dwt, (taps, C, C), 'conv_wgrad_ck8: dwt')
-    if not (1 <= taps <= 9 and taps % 2 == 1) or dilation < 0:
-        raise ValueError(f'conv_wgrad_ck8: an odd number of taps up to 9 and dilation >= 0, got {taps}, {dilation}')
+    if not (1 <= taps <= 9 and taps % 2 == 1) or not 0 <= dilation < 2 ** 31:
+        raise ValueError(f'conv_wgrad_ck8: an odd number of taps up to 9 and 0 <= dilation < 2^31, got {taps}, {dilation}')
     need = _lib.load().drk_conv_wgrad_ck8_workspace_bytes(B, L, taps, dilation)
     ws = _scratch(need, dc.device)
     _lib.call('drk_conv_wgrad_ck8', codes, exps, _at(gamma, f32, 'gamma', dev), _at(beta, f32, 'beta', dev),

@@ -67,13 +67,11 @@ class Interpolant:
         entropy and the `topk` most likely residues, at every position of the (partly masked) aatypes int64 [B, L].
         Positions outside `mask` and negative targets are not scored; the mask token is no answer; allowed: bool [22] or
         [B, L, 22], what else may stand there.  -> (logp, entropy, top_ids, top_logp), differentiable in the model."""
-        logits = model(X, aatypes, mask, chain_M, residue_idx, chain_encoding_all)
-        if logits.stride(-1) != 1:
-            logits = logits.contiguous()
+        logits = model(X, aatypes, mask, chain_M, residue_idx, chain_encoding_all).contiguous()
         answers = torch.arange(self.num_tokens, device=logits.device) != MASK_TOKEN_INDEX
         if allowed is not None:
-            answers = (answers & allowed).contiguous()
-        targets = torch.where(mask != 0, targets, torch.full_like(targets, -1))
+            answers = (answers & (allowed != 0)).contiguous()
+        targets = torch.where(mask != 0, targets, torch.full_like(targets, -1)).contiguous()
         return autograd.token_scores_with_grad(logits, targets, allowed=answers, temp=float(self._cfg.temp), topk=topk)
 
     def sample_gradient(self, model, X, mask, chain_M, residue_idx, chain_encoding_all, truncate_steps, gumbel_softmax_temp,

@@ -373,3 +373,12 @@ def test_refusals(dev):
     assert dce.shape == (0, 4, C)
     ops.conv_wgrad_ck8(eck, one, one, dc[:0], dwt, 1)
     assert float(dwt.abs().sum()) == 0
+
+
+@pytest.mark.gpu
+def test_a_dilation_beyond_an_int_is_refused(dev):
+    _, ck = ops.ln_fwd_ck8(torch.zeros(1, 4, C, device=dev), None, 0, None, None)
+    dc, dwt = torch.zeros(1, 4, C, dtype=torch.bfloat16, device=dev), torch.zeros(9, C, C, device=dev)
+    for dil in (2 ** 31, 2 ** 32 + 1):
+        with pytest.raises(ValueError):
+            ops.conv_wgrad_ck8(ck, None, None, dc, dwt, dil)

@@ -469,3 +469,57 @@ def test_interpolant_score_tokens(dev):
     assert bool((logp[1, 20:] == 0).all()) and not bool(((ids == 21) | (ids == 1)).any())
     logp[torch.isfinite(logp)].sum().backward()
     assert torch.isfinite(W.grad.float()).all() and float(W.grad[:, [1, 21]].abs().sum()) == 0
+
+
+@pytest.mark.gpu
+def test_more_rows_than_one_launch_holds(dev):
+    """2^26 + 3 rows of one wave each: more than 2^32 threads."""
+    rows, V = (1 << 26) + 3, 65
+    lg = torch.zeros(rows, V, dtype=torch.bfloat16, device=dev)
+    at = torch.tensor([0, (1 << 24) - 2, (1 << 24) - 1, 1 << 24, rows - 2, rows - 1])       # (a launch takes 2^24 - 1 rows)
+    lg[at.to(dev)] = torch.randn(6, V, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(dev)
+    part = lg[at.to(dev)]
+    tok = torch.full((rows,), 7, dtype=torch.int64, device=dev)
+    s = ops.token_scores(lg, tok, topk=1)
+    logp, H, ids, top, _, p = oracle(part, tok[:6], None, 1.0, 1)
+    close(s.logp[at.to(dev)], logp, 'logp')
+    close(s.entropy[at.to(dev)], H, 'entropy')
+    assert torch.equal(s.top_ids[at.to(dev)].cpu(), ids)
+    assert bool((s.stats[:, 1] > 0).all())                                                  # no row left out
+    d = ops.token_scores_bwd(lg, tok, s, g_logp=torch.ones(rows, device=dev), out=lg)
+    want = -p
+    want[:, 7] += 1
+    bar = torch.finfo(torch.bfloat16).eps / 2 * want.abs() + 256 * ULP
+    assert bool(((d[at.to(dev)].cpu().double() - want).abs() <= bar).all())
+    assert bool((d[:, 7] > 0).all())
+
+
+@pytest.mark.gpu
+def test_diffusion_score_tokens_keeps_no_tensor(dev, gpu_model):
+    """A tensor made by one call (on its stream, or inside its capture) is not another call's input."""
+    x = torch.full((1, 200), 4, dtype=torch.int64, device=dev)
+    held = set(vars(gpu_model))
+    with torch.no_grad():
+        gpu_model.score_tokens(x, torch.zeros(1, device=dev), x.clamp(max=3))
+    assert not [k for k in set(vars(gpu_model)) - held if isinstance(vars(gpu_model)[k], torch.Tensor)]
+
+
+@pytest.mark.gpu
+def test_interpolant_score_tokens_of_transposed_inputs(dev):
+    from types import SimpleNamespace as NS
+    from drakes_amd.protein import Interpolant
+    lg = torch.randn(31, 2, 22, generator=torch.Generator().manual_seed(3)).to(dev)
+    it = Interpolant(NS(num_timesteps=10, min_t=0.01, temp=0.5, interpolant_type='masking'))
+    tgt = torch.randint(0, 21, (31, 2), generator=torch.Generator().manual_seed(2)).to(dev)
+    mask = torch.ones(31, 2, device=dev)
+    mask[20:, 1] = 0
+    allowed = torch.full((22,), 2, dtype=torch.uint8, device=dev)
+    allowed[1] = 0
+    model = lambda X, S, *a: lg.transpose(0, 1)
+    logp, H, ids, _ = it.score_tokens(model, None, None, tgt.t(), mask.t(), None, None, None, topk=2, allowed=allowed)
+    on = allowed.cpu() != 0
+    on[21] = False
+    want = oracle(lg.transpose(0, 1), torch.where(mask != 0, tgt, torch.full_like(tgt, -1)).t(), on, 0.5, 2)
+    close(logp, want[0], 'logp')
+    close(H, want[1], 'entropy')
+    assert torch.equal(ids.cpu(), want[2])
