@@ -309,7 +309,8 @@ __global__ void __launch_bounds__(256) k_ck8_sums(const float* __restrict__ slab
 // A matrix product whose K runs along the rows: 128 ci x 128 co per tap, 294 912 operations per row at 9 taps against 388
 // bytes read, so it is bound by the matrix cores and by what feeds them.  Sequences follow each other without padding; a
 // 32-row step of a tap has the rows that stay in their sequence as 32 bits, computed from the step's first position; the
-// others are cleared in the xq fragment (an infinity or NaN of dc meets a zero there and makes NaN, as with padded rows).
+// others are cleared in the xq fragment (an infinity or NaN of dc meets a zero there and makes NaN, as with padded rows; a step
+// that k_wgrad_ck8_tap leaves out, since its tap reaches none of its rows, looks for one).
 // Both operands are read transposed (ds_read_b64_tr_b16) from tiles in LDS.  S comes from the same product: a fragment whose
 // row m is 1 where tap m is inside its sequence.
 //   k_wgrad_ck8_ring: all taps in one workgroup, 32 of the 128 input channels.  The decoded xq rows form a ring: every row is
@@ -390,6 +391,7 @@ __device__ __forceinline__ bf16v8 cw_clear(bf16v8 f, u32x4 mask) { return __buil
 __global__ void __launch_bounds__(256) k_wgrad_ck8_tap(CwArgs a) {
   __shared__ __attribute__((aligned(16))) char xs[2][CW_TILE * 128];      // xq, 64 channels
   __shared__ __attribute__((aligned(16))) char ds[2][CW_DC];
+  __shared__ unsigned nan_at[DRK_C / 2];                                  // two channels of dc each, as `lost`
   // the two halves of a chunk read the same dc: 8 workgroups apart they run on the same XCD
   const int half = (blockIdx.x >> 3) & 1, chunk = (blockIdx.x >> 4) * 8 + (blockIdx.x & 7);
   if (chunk >= a.chunks) return;
@@ -422,7 +424,20 @@ __global__ void __launch_bounds__(256) k_wgrad_ck8_tap(CwArgs a) {
       if (g < a.M) rd[i] = *(const f32x4*)(a.dc + g * 256 + 16 * (it & 15));
     }
   };
+  unsigned live[2];              // of the stored tile's two steps: the rows that stay in their sequence
+  u32x4 lost = {0u, 0u, 0u, 0u};      // bits 15, 31: dc of this thread's 8 channels was not finite in a step without such a row
   auto store = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      live[ks] = cw_inside(lb, L, shift);
+      lb += lstep;
+      lb -= lb >= L ? L : 0;
+      if (!live[ks]) {           // (rd[2 ks], rd[2 ks + 1] hold rows of step ks; an exponent of ones carries into the next bit)
+        const u32x4 d0 = __builtin_bit_cast(u32x4, rd[2 * ks]), d1 = __builtin_bit_cast(u32x4, rd[2 * ks + 1]);
+        lost |= ((d0 & 0x7f807f80u) + 0x00800080u) | ((d1 & 0x7f807f80u) + 0x00800080u);
+      }
+    }
+    if (!(live[0] | live[1])) return;                      // nobody reads this tile
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int it = tid + 256 * i, row = it >> 3;
@@ -445,6 +460,7 @@ __global__ void __launch_bounds__(256) k_wgrad_ck8_tap(CwArgs a) {
 #pragma unroll
   for (int n = 0; n < 4; ++n) acc[0][n] = acc[1][n] = f32x4{0.f, 0.f, 0.f, 0.f};
   accs[0] = accs[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (tid < 64) nan_at[tid] = 0u;
   fetch(0);
   store(0);
   __syncthreads();
@@ -453,7 +469,7 @@ __global__ void __launch_bounds__(256) k_wgrad_ck8_tap(CwArgs a) {
     const char *xt = xs[T & 1], *dt = ds[T & 1];
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      const unsigned rows = cw_inside(lb, L, shift);
+      const unsigned rows = live[ks];
       if (rows) {
         bf16v8 af[2], bf[4];
 #pragma unroll
@@ -474,24 +490,31 @@ __global__ void __launch_bounds__(256) k_wgrad_ck8_tap(CwArgs a) {
             accs[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16v8, mask), ciq ? bf[2 + n] : bf[n], accs[n], 0, 0, 0);
         }
       }
-      lb += lstep;
-      lb -= lb >= L ? L : 0;
     }
-    if (T + 1 < c.nt) store((T + 1) & 1);                  // its last readers passed the previous barrier
+    if (T + 1 < c.nt) {
+      store((T + 1) & 1);                                  // its last readers passed the previous barrier
+    } else {
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+        if (lost[d] & 0x80008000u) atomicOr(&nan_at[4 * (tid & 15) + d], lost[d] & 0x80008000u);
+    }
     __syncthreads();
   }
   // D[row 4 g + v][col] of tile (m, n): ci = 64 half + 32 ciq + 16 m + 4 g + v, co = 64 coh + 16 n + (lane & 15)
   float* dst = a.slabs + ((long)chunk * a.taps + tap) * CW_SLAB;
   const int g = lane >> 4, cn = lane & 15;
+  bool nan[4];
+#pragma unroll
+  for (int n = 0; n < 4; ++n) nan[n] = (nan_at[(64 * coh + 16 * n + cn) >> 1] >> (cn & 1 ? 31 : 15)) & 1u;
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
     for (int n = 0; n < 4; ++n)
 #pragma unroll
-      for (int v = 0; v < 4; ++v) dst[(64 * half + 32 * ciq + 16 * m + 4 * g + v) * DRK_C + 64 * coh + 16 * n + cn] = acc[m][n][v];
+      for (int v = 0; v < 4; ++v) dst[(64 * half + 32 * ciq + 16 * m + 4 * g + v) * DRK_C + 64 * coh + 16 * n + cn] = nan[n] ? NAN : acc[m][n][v];
   if (half == 0 && g == 0) {
 #pragma unroll
-    for (int n = 0; n < 2; ++n) dst[DRK_C * DRK_C + 64 * coh + 16 * (2 * ciq + n) + cn] = accs[n][0];
+    for (int n = 0; n < 2; ++n) dst[DRK_C * DRK_C + 64 * coh + 16 * (2 * ciq + n) + cn] = (ciq ? nan[2 + n] : nan[n]) ? NAN : accs[n][0];
   }
 }
 

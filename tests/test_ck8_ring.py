@@ -58,3 +58,28 @@ def test_ring(dev, B, L, taps, dil, affine):
     again = torch.full((taps, C, C), 0.25, device=dev)
     ops.conv_wgrad_ck8(ck, up(gamma), up(beta), dc.to(dev), again, dil)
     assert torch.equal(again, dwt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('B,L,taps,dil', [(32, 200, 9, 64), (70, 200, 9, 64), (63, 200, 9, 16), (65, 200, 9, 16), (3, 33, 9, 4), (2, 7, 9, 9),
+                                          (1, 1, 3, 1), (2, 1024, 9, 64), (13, 1024, 9, 105), (5, 40, 1, 0)])
+@pytest.mark.parametrize('bad', [math.nan, math.inf, -math.inf])
+def test_a_nan_or_an_infinity_in_dc_reaches_every_tap(dev, B, L, taps, dil, bad):
+    """As where h is padded with zeros: the row meets a zero in a tap that leaves its sequence.  Whichever kernel runs."""
+    ck, _ = checkpoint(B + L, B, L, dev)
+    gamma, beta = (1 + 0.2 * rnd(1, C)).to(dev), (0.5 * rnd(2, C)).to(dev)
+    dc = (rnd(3, B, L, C) * (rnd(4, B, L, C) > 0)).to(torch.bfloat16)
+    at = [(0, 0, 0), (B // 2, L // 2, 77), (B - 1, L - 1, 127), (B - 1, 0, 6)]
+    cols = [c for _, _, c in at]
+    out = []
+    for v in (0.0, bad):
+        for b, l, c in at:
+            dc[b, l, c] = v
+        dwt = torch.zeros(taps, C, C, device=dev)
+        ops.conv_wgrad_ck8(ck, gamma, beta, dc.to(dev), dwt, dil)
+        out.append(dwt.cpu())
+    clean, got = out
+    assert torch.isfinite(clean).all()
+    assert not torch.isfinite(got[:, :, cols]).any(), [(t, c) for t in range(taps) for c in cols if torch.isfinite(got[t, :, c]).any()]
+    rest = [c for c in range(C) if c not in cols]
+    assert torch.equal(got[:, :, rest], clean[:, :, rest])
