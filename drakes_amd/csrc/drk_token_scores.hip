@@ -264,8 +264,8 @@ __device__ __forceinline__ TsRowGrad ts_row_grad(const TsBwdArgs& a, long row) {
   return g;
 }
 __device__ __forceinline__ float ts_dense_grad(float x, const TsRowGrad& g, float inv_temp) {
-  const float lp = (x - g.m) * inv_temp - g.ls, p = ts_exp2(lp * TS_LOG2E);
-  return x == -INFINITY ? 0.f : -p * (g.whole + g.gh * (ts_factor(lp) + g.H));
+  const float lp = (x - g.m) * inv_temp - g.ls, p = ts_exp2(lp * TS_LOG2E);      // (p is 0 from lp = -128 on)
+  return x == -INFINITY ? 0.f : -p * (g.whole + g.gh * (fmaxf(lp, -128.f) + g.H));
 }
 
 template <class D, bool VEC>
