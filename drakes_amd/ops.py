@@ -6,7 +6,6 @@ falls back to torch kernels.
 """
 import collections
 import ctypes
-import math
 
 import torch
 
@@ -612,6 +611,7 @@ def reverse_step_soft_wide_bwd(logits, x_soft, grad_x_next, grad_flag, d_t, move
 
 # ---- scores of given tokens ------------------------------------------------------------------------
 TOPK_MAX = 32
+TEMP_MIN, TEMP_MAX = 1e-38, 1e26
 _SCORE_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 # logp [...], entropy [...] or None, top_ids / top_logp [..., k] or None, stats [..., 2] (what the backward needs)
@@ -673,8 +673,8 @@ def _score_args(name, logits, tokens, allowed, temp):
         raise TypeError(f'{name}: logits are float32, bfloat16 or float16, got {logits.dtype}')
     if logits.ndim < 1 or logits.shape[-1] < 1 or tokens.shape != logits.shape[:-1]:
         raise ValueError(f'{name}: logits [..., V] and tokens [...], got {tuple(logits.shape)} and {tuple(tokens.shape)}')
-    if not 0.0 < temp < math.inf:
-        raise ValueError(f'{name}: temp must be positive, got {temp}')
+    if not TEMP_MIN <= temp <= TEMP_MAX:
+        raise ValueError(f'{name}: temp must be in [{TEMP_MIN}, {TEMP_MAX}], got {temp}')
     dev, stream = _current()
     if logits.get_device() != dev:
         raise ValueError(f'{name}: logits on {logits.device}, but the current device is cuda:{dev}')

@@ -113,7 +113,7 @@ int drk_likelihood_accum(const float* logits, const int64_t* x0, const int64_t* 
  * logits: rows of V values of type `dtype`, row r at logits + r * row_stride values (row_stride 0: one row for all);
  * tokens int64 [rows].  A column counts when allowed is NULL or allowed[r * allowed_stride + j] != 0 (uint8;
  * allowed_stride 0: one list for all rows, else >= V) and its logit is not -inf; what stands in other columns is never
- * looked at.  With p = softmax over those columns of logits / temp (0 < temp < inf):
+ * looked at.  With p = softmax over those columns of logits / temp (DRK_TEMP_MIN <= temp <= DRK_TEMP_MAX):
  *   logp [rows]: log p(token); 0 for a negative token (not scored), -inf for a column that does not count, NaN for a
  *                token >= V;
  *   entropy [rows] (optional): -sum p log p, in nats;
@@ -126,6 +126,8 @@ int drk_likelihood_accum(const float* logits, const int64_t* x0, const int64_t* 
 #define DRK_BF16 1
 #define DRK_F16 2
 #define DRK_TOPK_MAX 32
+#define DRK_TEMP_MIN 1e-38f
+#define DRK_TEMP_MAX 1e26f
 int drk_token_scores(const void* logits, int dtype, long row_stride, const int64_t* tokens, const unsigned char* allowed,
                      long allowed_stride, float temp, int k, float* logp, float* entropy, int64_t* top_ids,
                      float* top_logp, float* stats, long rows, int V, void* workspace, long workspace_bytes, void* stream);

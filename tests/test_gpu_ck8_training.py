@@ -205,3 +205,62 @@ def test_fine_tune_sampler_and_refusals(dev, det_sd):
     lp.backward(retain_graph=True)
     with pytest.raises(RuntimeError):
         lp.backward()
+
+
+def _input_gradient_in_torch(fn, m, dlogits):
+    """dL/dseq from the node's checkpoints, gates and statistics, with the kernels' bf16 rounding points."""
+    bb = m.backbone
+    P = {k: p.detach() for k, p in bb.named_parameters()}
+    n = bb.num_layers
+    conv = lambda dc, w, d: torch.nn.functional.conv_transpose1d(dc.transpose(1, 2).double(), w.bfloat16().double(), padding=(w.shape[2] // 2) * d, dilation=d).transpose(1, 2).float()
+    mean = lambda t: t.mean(-1, keepdim=True)
+    dpre = (dlogits @ P['final_conv.2.weight'].squeeze(-1)) * (fn.y > 0)
+    gr = conv(dpre.bfloat16().float(), P['final_conv.0.weight'], 1)
+    up = gr * _open(fn.kept[n].gates)
+    for i in reversed(range(n)):
+        dh = conv(up.bfloat16().float(), P[f'convs.{i}.weight'], bb.dilation(i))
+        a, xq = dh * P[f'norms.{i}.weight'], ops.ck8_unpack(fn.kept[i])
+        gr = gr + fn.kept[i].rstd.unsqueeze(-1) * (a - mean(a) - xq * mean(a * xq))
+        up = gr * _open(fn.kept[i].gates)
+    w = P['linear.weight'].double()
+    return torch.nn.functional.conv_transpose1d(up.transpose(1, 2).double(), w, padding=w.shape[2] // 2).transpose(1, 2)
+
+
+@pytest.mark.parametrize('B,L', [(3, 77), (33, 200), (1, 3), (70, 200), (2, 1024)])
+@pytest.mark.parametrize('frozen', [False, True])
+def test_input_gradient_equals_the_formulas_on_the_checkpoints(dev, det_sd, B, L, frozen):
+    """Bar (1) of the head: the input gradient is the last of the tensors that the same chain of roundings reaches."""
+    m = _model(dev, det_sd, length=L)
+    if frozen:
+        m.requires_grad_(False)
+    g = torch.Generator().manual_seed(B)
+    seq = torch.softmax(torch.randn(B, L, 5, generator=g), -1).to(dev).requires_grad_()
+    logits = autograd.backbone_with_grad(m.backbone, seq, torch.zeros(1, device=dev), 'bf16', keep='int8')
+    dlogits = torch.randn(B, L, 5, generator=g).to(dev)
+    want = _input_gradient_in_torch(logits.grad_fn, m, dlogits)
+    logits.backward(dlogits)
+    err = float((seq.grad.double() - want).norm())
+    assert err <= 7.5e-3 * float(want.norm()), (err, float(want.norm()))
+
+
+@pytest.mark.parametrize('B,L', [(32, 200), (70, 200), (4, 1024)])
+def test_gradients_stay_within_a_few_percent_of_the_path_without_checkpoints(dev, det_sd, B, L):
+    """Bar (2) of the head taken per block of 32 channels: a block's largest magnitude is at most sqrt(32) of its rms, so a kept
+    value's error has an rms of at most 5.7 / 63.5 / sqrt(12) = 0.026 of the block's; both a weight gradient and its error are
+    sums over the same rows.  With a LayerNorm backward of 0.026 / sqrt(128) at each of 20 layers (0.010) and two forwards' bf16
+    roundings (0.02), in quadrature 0.034: 0.04.  Over all parameters, whose blocks are not all at that extreme: half of it."""
+    m = _model(dev, det_sd, length=L)
+    x = torch.randint(0, 5, (B, L), generator=torch.Generator().manual_seed(1)).to(dev)
+    tgt = torch.randint(0, 4, (B, L), generator=torch.Generator().manual_seed(2)).to(dev)
+    only = torch.where(x == 4, tgt, torch.full_like(tgt, -1))
+    out = {}
+    for keep in (None, 'int8'):
+        m.hip_checkpoint = keep
+        (-m.score_tokens(x, torch.zeros(B, device=dev), only)[0].sum() / (x == 4).sum()).backward()
+        out[keep] = _grads(m)
+    a, b = out[None], out['int8']
+    rel = {k: float((a[k] - b[k]).norm()) / float(a[k].norm()) for k in a}
+    worst = max(rel, key=rel.get)
+    print(f'worst {worst} {rel[worst]:.4f}, median {sorted(rel.values())[len(rel) // 2]:.4f}')
+    assert rel[worst] < 0.04, (worst, rel[worst])
+    assert sorted(rel.values())[len(rel) // 2] < 0.02
