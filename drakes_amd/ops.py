@@ -611,6 +611,7 @@ def reverse_step_soft_wide_bwd(logits, x_soft, grad_x_next, grad_flag, d_t, move
 
 # ---- scores of given tokens ------------------------------------------------------------------------
 TOPK_MAX = 32
+V_MAX = 1 << 30
 TEMP_MIN, TEMP_MAX = 1e-38, 1e26
 _SCORE_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -673,6 +674,8 @@ def _score_args(name, logits, tokens, allowed, temp):
         raise TypeError(f'{name}: logits are float32, bfloat16 or float16, got {logits.dtype}')
     if logits.ndim < 1 or logits.shape[-1] < 1 or tokens.shape != logits.shape[:-1]:
         raise ValueError(f'{name}: logits [..., V] and tokens [...], got {tuple(logits.shape)} and {tuple(tokens.shape)}')
+    if logits.shape[-1] > V_MAX:               # (V and the columns' numbers are 32-bit: a larger one would wrap on the way)
+        raise ValueError(f'{name}: at most 2^30 columns, got {logits.shape[-1]}')
     if not TEMP_MIN <= temp <= TEMP_MAX:
         raise ValueError(f'{name}: temp must be in [{TEMP_MIN}, {TEMP_MAX}], got {temp}')
     dev, stream = _current()

@@ -109,7 +109,7 @@ int drk_q_xt(const int64_t* x0, const float* uniforms, int64_t* xt, int B, int L
 int drk_likelihood_accum(const float* logits, const int64_t* x0, const int64_t* xt, float multiplier, float* acc,
                          int B, int L, void* stream);
 
-/* ---- scores of given tokens: log-probability, entropy, top alternatives, any vocabulary --------------------------
+/* ---- scores of given tokens: log-probability, entropy, top alternatives, vocabularies of up to 2^30 ----------------
  * logits: rows of V values of type `dtype`, row r at logits + r * row_stride values (row_stride 0: one row for all);
  * tokens int64 [rows].  A column counts when allowed is NULL or allowed[r * allowed_stride + j] != 0 (uint8;
  * allowed_stride 0: one list for all rows, else >= V) and its logit is not -inf; what stands in other columns is never

@@ -71,3 +71,15 @@ def test_temperatures_out_of_range_are_refused_from_python(dev):
             ops.token_scores(lg, tok, temp=t)
         with pytest.raises(ValueError, match='temp'):
             ops.token_scores_bwd(lg, tok, s, temp=t)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('V', [2 ** 30 + 1, 2 ** 31 + 7, 2 ** 32 + 7])
+def test_a_vocabulary_beyond_the_limit_is_refused(dev, V):
+    """Not scored over its first V mod 2^32 columns.  (No row, so nothing is allocated or launched.)"""
+    lg, tok = torch.empty(0, V, dtype=torch.float16, device=dev), torch.empty(0, dtype=torch.int64, device=dev)
+    with pytest.raises(ValueError, match='2\\^30'):
+        ops.token_scores(lg, tok)
+    e = torch.empty(0, device=dev)
+    with pytest.raises(ValueError, match='2\\^30'):
+        ops.token_scores_bwd(lg, tok, ops.TokenScores(e, e, None, None, torch.empty(0, 2, device=dev)), g_logp=e)
