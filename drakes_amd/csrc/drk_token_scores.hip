@@ -287,6 +287,8 @@ __global__ void __launch_bounds__(64) k_scores_small_bwd(TsBwdArgs a) {
       const float gr = a.g_top[row * a.k + r];
       g.whole += j >= 0 ? gr : 0.f;
     }
+    // (a row with NaN has a NaN for a token that does not count: its column gets nothing all the same)
+    if (g.g1 != 0.f && (!((on >> g.t) & 1) || lds[ts_pad(base + (int)g.t)] == -INFINITY)) g.g1 = 0.f;
     for (int j = 0; j < V; j += 8) {
       float x[8];
       ts_eight(lds, base, j, V, on, x);
@@ -690,7 +692,8 @@ __global__ void __launch_bounds__(T) k_scores_row_bwd(TsBwdArgs a) {
     if (mine >= a.V) mine = -1;
     else if (mine < R.head || mine >= R.tail) mine = part == 0 ? mine : -1;
     else if ((mine - R.head) / E < c0 || (mine - R.head) / E >= c1) mine = -1;
-    if (mine >= 0) xm = D::get(R.x[mine]);
+    if (mine >= 0) xm = R.one(mine);
+    if (xm == -INFINITY) hot = 0.f;          // (the token of a row with NaN may be one that does not count)
   }
   const int je = part == 0 ? R.edge(tid) : -1;
   const float xe = R.one(je);

@@ -83,3 +83,24 @@ def test_a_vocabulary_beyond_the_limit_is_refused(dev, V):
     e = torch.empty(0, device=dev)
     with pytest.raises(ValueError, match='2\\^30'):
         ops.token_scores_bwd(lg, tok, ops.TokenScores(e, e, None, None, torch.empty(0, 2, device=dev)), g_logp=e)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('V', [7, 64, 65, 1001, 9001, 140001])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('shared', [True, False])
+def test_columns_that_do_not_count_get_no_gradient_in_a_row_with_nan(dev, V, dtype, shared):
+    """The given token is one of them, and its log-probability is the row's NaN."""
+    for t in (0, V // 3, V - 1):
+        lg = torch.randn(2, V, generator=torch.Generator().manual_seed(V)).to(dtype)
+        lg[:, (t + 2) % V] = math.nan
+        allowed = torch.ones(V, dtype=torch.bool)
+        allowed[t] = False
+        al = (allowed if shared else allowed.expand(2, V).contiguous()).to(dev)
+        tok = torch.full((2,), t, device=dev)
+        s = ops.token_scores(lg.to(dev), tok, allowed=al, topk=2)
+        assert torch.isnan(s.logp).all()
+        one = torch.ones(2, device=dev)
+        d = ops.token_scores_bwd(lg.to(dev), tok, s, g_logp=one, g_entropy=one, g_top=torch.ones(2, 2, device=dev), allowed=al).cpu()
+        assert bool((d[:, t] == 0).all()), d[:, t]
+        assert torch.isnan(d[:, allowed]).all()
