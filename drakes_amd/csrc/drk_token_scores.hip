@@ -246,7 +246,8 @@ struct TsBwdArgs {
   float inv_temp;
 };
 
-// What a row's gradient is made of: d_j = inv_temp * (hot_j - p_j * (whole + gh * (logp_j + H)))
+// What a row's gradient is made of: d_j = inv_temp * (hot_j - p_j * (whole + gh * (logp_j + H))).  A row into which nothing
+// comes gets zeros whatever its p, which may be NaN: a batch's padding may hold anything.
 struct TsRowGrad {
   float m, ls, gh, H, g1, whole;
   int64_t t;
@@ -281,14 +282,17 @@ __global__ void __launch_bounds__(64) k_scores_small_bwd(TsBwdArgs a) {
   __syncthreads();
   if (row < a.rows) {
     TsRowGrad g = ts_row_grad(a, row);
+    bool any = g.g1 != 0.f || g.gh != 0.f;
 #pragma unroll 4
     for (int r = 0; r < a.k; ++r) {
       const int64_t j = a.top_ids[row * a.k + r];
-      const float gr = a.g_top[row * a.k + r];
-      g.whole += j >= 0 ? gr : 0.f;
+      const float gr = j >= 0 ? a.g_top[row * a.k + r] : 0.f;
+      g.whole += gr;
+      any |= gr != 0.f;
     }
     // (a row with NaN has a NaN for a token that does not count: its column gets nothing all the same)
-    if (g.g1 != 0.f && (!((on >> g.t) & 1) || lds[ts_pad(base + (int)g.t)] == -INFINITY)) g.g1 = 0.f;
+    const int tc = g.g1 != 0.f ? (int)g.t : 0;
+    const float xt = (on >> tc) & 1 ? lds[ts_pad(base + tc)] : -INFINITY;
     for (int j = 0; j < V; j += 8) {
       float x[8];
       ts_eight(lds, base, j, V, on, x);
@@ -296,7 +300,9 @@ __global__ void __launch_bounds__(64) k_scores_small_bwd(TsBwdArgs a) {
       for (int u = 0; u < 8; ++u)
         if (j + u < V) lds[ts_pad(base + j + u)] = ts_dense_grad(x[u], g, a.inv_temp) * a.inv_temp;
     }
-    if (g.g1 != 0.f) lds[ts_pad(base + (int)g.t)] += g.g1 * a.inv_temp;
+    if (!any)
+      for (int j = 0; j < V; ++j) lds[ts_pad(base + j)] = 0.f;
+    if (g.g1 != 0.f && xt != -INFINITY) lds[ts_pad(base + (int)g.t)] += g.g1 * a.inv_temp;
     for (int r = 0; r < a.k; ++r) {
       const int64_t j = a.top_ids[row * a.k + r];
       if (j >= 0 && j < V) lds[ts_pad(base + (int)j)] += a.g_top[row * a.k + r] * a.inv_temp;
@@ -680,6 +686,7 @@ __global__ void __launch_bounds__(T) k_scores_row_bwd(TsBwdArgs a) {
     gr = id >= 0 ? a.g_top[row * a.k + lane] : 0.f;
   }
   if (a.k) g.whole += ts_wave(gr, [](float u, float v) { return u + v; });
+  const bool none = g.g1 == 0.f && g.gh == 0.f && !__ballot(gr != 0.f);
   // thread r < k stores alternative r's column once more, thread k the given token's: what the one-hot terms add to it
   int mine = tid < a.k ? id : tid == a.k && g.g1 != 0.f ? (int)g.t : -1;
   float xm = -INFINITY, hot = mine >= 0 && mine == g.t ? g.g1 : 0.f;
@@ -692,8 +699,11 @@ __global__ void __launch_bounds__(T) k_scores_row_bwd(TsBwdArgs a) {
     if (mine >= a.V) mine = -1;
     else if (mine < R.head || mine >= R.tail) mine = part == 0 ? mine : -1;
     else if ((mine - R.head) / E < c0 || (mine - R.head) / E >= c1) mine = -1;
-    if (mine >= 0) xm = R.one(mine);
-    if (xm == -INFINITY) hot = 0.f;          // (the token of a row with NaN may be one that does not count)
+    if (mine >= 0) {
+      xm = D::get(R.x[mine]);
+      if (R.al && !R.al[mine]) xm = -INFINITY;
+      if (xm == -INFINITY) hot = 0.f;        // (the token of a row with NaN may be one that does not count)
+    }
   }
   const int je = part == 0 ? R.edge(tid) : -1;
   const float xe = R.one(je);
@@ -718,6 +728,11 @@ __global__ void __launch_bounds__(T) k_scores_row_bwd(TsBwdArgs a) {
     }
   }
   __syncthreads();
+  if (none) {
+    if (je >= 0) dx[je] = D::put(0.f);
+    for (long i = R.head + (long)c0 * E + tid; i < R.head + (long)c1 * E; i += T) dx[i] = D::put(0.f);
+    return;
+  }
   if (mine >= 0) dx[mine] = D::put((ts_dense_grad(xm, g, a.inv_temp) + hot) * a.inv_temp);
 }
 

@@ -104,3 +104,27 @@ def test_columns_that_do_not_count_get_no_gradient_in_a_row_with_nan(dev, V, dty
         d = ops.token_scores_bwd(lg.to(dev), tok, s, g_logp=one, g_entropy=one, g_top=torch.ones(2, 2, device=dev), allowed=al).cpu()
         assert bool((d[:, t] == 0).all()), d[:, t]
         assert torch.isnan(d[:, allowed]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('V', [5, 22, 64, 65, 1001, 9001, 140001])
+@pytest.mark.parametrize('bad', [math.nan, math.inf])
+def test_rows_that_are_not_scored_pass_no_gradient_whatever_they_hold(dev, V, bad):
+    """The padding of a batch: negative tokens, and logits that came from nothing."""
+    x = torch.randn(6, V, generator=torch.Generator().manual_seed(V))
+    x[2:4] = bad
+    x[4, V // 2] = bad
+    tok = torch.tensor([1, 0, -1, -1, -1, V - 1], device=dev)
+    ref = x.clone()
+    ref[2:5] = 0.0
+    out = []
+    for lg in (x, ref):
+        s = ops.token_scores(lg.to(dev), tok)
+        out.append(ops.token_scores_bwd(lg.to(dev), tok, s, g_logp=torch.full((6,), 0.5, device=dev),
+                                        g_entropy=torch.tensor([1.0, 1, 0, 0, 0, 1], device=dev)).cpu())
+    got, want = out
+    assert bool((got[2:5] == 0).all())
+    assert torch.equal(got, want)
+    live = x.to(dev).requires_grad_()
+    drakes_amd.autograd.token_scores_with_grad(live, tok)[0].sum().backward()
+    assert torch.isfinite(live.grad).all() and bool((live.grad[2:5] == 0).all())
