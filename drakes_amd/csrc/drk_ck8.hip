@@ -597,7 +597,8 @@ __global__ void __launch_bounds__(512) k_wgrad_ck8_ring(CwArgs a) {
   const int co0 = 2 * tg + cih, co1 = co0 ^ 1, co2 = 2 * (1 - tg);   // b[0], b[1], b[2] (b[3] is the tile after b[2])
   const unsigned boff = dcs + (4 * kg + q) * CW_RD + 128 * coh + 8 * p, boff0 = boff + 32 * co0, boff1 = boff + 32 * co1, boff2 = boff + 32 * co2;
   struct Frags { bf16v8 a[CW_NT], b[4]; };
-  // (addresses are offsets into LDS: smem is all that this kernel has there, so it starts at 0)
+  // (addresses are offsets into LDS: smem is all that this kernel has there, so it starts at 0, which the host checks before the
+  // first launch; as offsets from a pointer they cost 1 % more time, an addition each)
   auto frag = [&](unsigned at, int second) __attribute__((always_inline)) {
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)at);
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)(at + second));
@@ -883,6 +884,10 @@ extern "C" int drk_conv_wgrad_ck8(const signed char* codes, const unsigned char*
     hipError_t e = hipGetDevice(&dev);
     if (e != hipSuccess) return drk_set_error(e, "drk_conv_wgrad_ck8(hipGetDevice)");
     if (dev < 0 || dev >= DRK_MAX_DEVICES || !lds_set[dev].load(std::memory_order_acquire)) {
+      hipFuncAttributes at;
+      e = hipFuncGetAttributes(&at, (const void*)k_wgrad_ck8_ring);
+      if (e != hipSuccess) return drk_set_error(e, "drk_conv_wgrad_ck8(hipFuncGetAttributes)");
+      if (at.sharedSizeBytes != 0) return drk_set_error_msg(DRK_EINVAL, "drk_conv_wgrad_ck8: this build's kernel has static LDS, its addresses take the ring to start at 0");
       e = hipFuncSetAttribute((const void*)k_wgrad_ck8_ring, hipFuncAttributeMaxDynamicSharedMemorySize, CW_RING_LDS(CW_RING_MAX));
       if (e != hipSuccess) return drk_set_error(e, "drk_conv_wgrad_ck8(LDS size)");
       if (dev >= 0 && dev < DRK_MAX_DEVICES) lds_set[dev].store(1u, std::memory_order_release);
