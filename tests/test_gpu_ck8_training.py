@@ -241,3 +241,26 @@ def test_input_gradient_equals_the_formulas_on_the_checkpoints(dev, det_sd, B, L
     logits.backward(dlogits)
     err = float((seq.grad.double() - want).norm())
     assert err <= 7.5e-3 * float(want.norm()), (err, float(want.norm()))
+
+
+@pytest.mark.parametrize('B,L', [(32, 200), (70, 200), (4, 1024)])
+def test_gradients_stay_within_a_few_percent_of_the_path_without_checkpoints(dev, det_sd, B, L):
+    """Bar (2) of the head taken per block of 32 channels: a block's largest magnitude is at most sqrt(32) of its rms, so a kept
+    value's error has an rms of at most 5.7 / 63.5 / sqrt(12) = 0.026 of the block's; both a weight gradient and its error are
+    sums over the same rows.  With a LayerNorm backward of 0.026 / sqrt(128) at each of 20 layers (0.010) and two forwards' bf16
+    roundings (0.02), in quadrature 0.034: 0.04.  Over all parameters, whose blocks are not all at that extreme: half of it."""
+    m = _model(dev, det_sd, length=L)
+    x = torch.randint(0, 5, (B, L), generator=torch.Generator().manual_seed(1)).to(dev)
+    tgt = torch.randint(0, 4, (B, L), generator=torch.Generator().manual_seed(2)).to(dev)
+    only = torch.where(x == 4, tgt, torch.full_like(tgt, -1))
+    out = {}
+    for keep in (None, 'int8'):
+        m.hip_checkpoint = keep
+        (-m.score_tokens(x, torch.zeros(B, device=dev), only)[0].sum() / (x == 4).sum()).backward()
+        out[keep] = _grads(m)
+    a, b = out[None], out['int8']
+    rel = {k: float((a[k] - b[k]).norm()) / float(a[k].norm()) for k in a}
+    worst = max(rel, key=rel.get)
+    print(f'worst {worst} {rel[worst]:.4f}, median {sorted(rel.values())[len(rel) // 2]:.4f}')
+    assert rel[worst] < 0.04, (worst, rel[worst])
+    assert sorted(rel.values())[len(rel) // 2] < 0.02
