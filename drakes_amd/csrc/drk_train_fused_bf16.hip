@@ -337,11 +337,14 @@ struct TrainBwdArgs {
 // else dx = dh (final_conv.0 has no LayerNorm in front of it).  gr += dx.  If mask_n is given: dc_next = bf16(gr * gate)
 // -> the LDS image (the next convolution's operand).  Column sums -> this wave's partial slab.
 // Register budget (gr, acc and the prefetched weight ring are live throughout: 144): the LayerNorm's input is requested
-// here, not under the taps, and folded away tile by tile — after pass 1 gr holds gr + rstd * dyg and acc holds
-// rstd * xhat, so pass 2 is gr -= rstd * m1 + acc * m2 and nothing else of the tile is kept; the per-channel vectors are
-// re-read from LDS per tile; dgamma / dbeta leave before the barrier.
+// here, not under the taps, and folded away tile by tile — after pass 1 gr holds gr + rstd * dyg and xr holds
+// rstd * xhat, so pass 2 is gr -= rstd * m1 + xr * m2 and nothing else of the tile is kept; the per-channel vectors are
+// re-read from LDS per tile; dgamma / dbeta leave before the barrier.  What lives across tiles and layers is held as single
+// floats: of f32x4 values that are worked on element by element (there is no packed fp32 arithmetic) the allocator kept
+// quadruples with one live element and spilled 160 registers; it is 42 now, and a fine-tune pass at B = 128 takes 59.5 ms
+// instead of 65.6 (B = 32: 46.5 and 49.8).
 template <int NT, bool LN, bool FAST>
-__device__ __forceinline__ void epilogue_lnb(char* smem, f32x4 (&gr)[NT][2], f32x4 (&acc)[NT][2], const float* feat_i, bool feat_rows,
+__device__ __forceinline__ void epilogue_lnb(char* smem, float (&gr)[NT][2][4], f32x4 (&acc)[NT][2], const float* feat_i, bool feat_rows,
                                              const float* gamma, const float* tbv_src, int L, int lane, int ct, int grp,
                                              const unsigned long long* mask_n, float* part_o, const float* mean_nx,
                                              const float* rstd_nx, int tid, char* dc_o, const float* stat, float* stat_nx,
@@ -371,7 +374,9 @@ __device__ __forceinline__ void epilogue_lnb(char* smem, f32x4 (&gr)[NT][2], f32
       *(f32x4*)(part_o + ch0 + q * 128 + 16) = v1;
     }
   };
-  f32x4 sx0 = zero4, sx1 = zero4;
+  float sx[2][4] = {}, sc[2][4] = {};
+  auto quad = [](const float (&v)[4]) __attribute__((always_inline)) { return f32x4{v[0], v[1], v[2], v[3]}; };
+  float xr[NT][2][4];              // rstd * xhat
   if constexpr (LN) {
     f32x4 xh[NT][2];
     // (requested here, not under the taps: 56 more live registers there spill, and in flight under the taps they were
@@ -412,12 +417,16 @@ __device__ __forceinline__ void epilogue_lnb(char* smem, f32x4 (&gr)[NT][2], f32
       const float s1 = (sv[0] + sv[1]) + (sv[2] + sv[3]);
       const float s2 = (qv[0] + qv[1]) + (qv[2] + qv[3]);
       const f32x4 a0 = y0 * rs, a1 = y1 * rs;
-      gr[t][0] += a0;
-      gr[t][1] += a1;
-      sx0 += a0;
-      sx1 += a1;
-      acc[t][0] = h0 * rs;
-      acc[t][1] = h1 * rs;
+      const f32x4 x0 = h0 * rs, x1 = h1 * rs;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        gr[t][0][i] += a0[i];
+        gr[t][1][i] += a1[i];
+        sx[0][i] += a0[i];
+        sx[1][i] += a1[i];
+        xr[t][0][i] = x0[i];
+        xr[t][1][i] = x1[i];
+      }
       const u32x2 sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(s1), __float_as_uint(s2), false, false);
       y[t] = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
     }
@@ -439,10 +448,13 @@ __device__ __forceinline__ void epilogue_lnb(char* smem, f32x4 (&gr)[NT][2], f32
       const int p = 16 * (grp + 2 * t) + pn;
       const bool ok = (FAST && grp + 2 * t < 12) || p < L;
       const f32x4 d0 = ok ? acc[t][0] : zero4, d1 = ok ? acc[t][1] : zero4;
-      gr[t][0] += d0;
-      gr[t][1] += d1;
-      sx0 += d0;
-      sx1 += d1;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        gr[t][0][i] += d0[i];
+        gr[t][1][i] += d1[i];
+        sx[0][i] += d0[i];
+        sx[1][i] += d1[i];
+      }
     }
     if (part_o) {
       put_sum(zero4, zero4, 0);
@@ -464,7 +476,6 @@ __device__ __forceinline__ void epilogue_lnb(char* smem, f32x4 (&gr)[NT][2], f32
   }
   if (dc_o) image_rows_out(smem, dc_o, L, tid);   // this layer's dc (the image until the barrier) -> its block, for the weight gradient
   __syncthreads();   // partials visible; every wave is past its reads of the dc image
-  f32x4 sc0 = zero4, sc1 = zero4;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int p = 16 * (grp + 2 * t) + pn;
@@ -474,22 +485,28 @@ __device__ __forceinline__ void epilogue_lnb(char* smem, f32x4 (&gr)[NT][2], f32
       const float m1 = ((q1[0] + q1[1]) + (q1[2] + q1[3])) * (1.0f / 128.0f);
       const float m2 = ((q2[0] + q2[1]) + (q2[2] + q2[3])) * (1.0f / 128.0f);
       const float c1 = stat[MAXPOS + p] * m1;
-      const f32x4 e0 = acc[t][0] * m2 + c1, e1 = acc[t][1] * m2 + c1;
       const bool ok = (FAST && grp + 2 * t < 12) || p < L;      // (rows >= L: acc holds rstd * xhat of a zero row, dyg = 0, m1 = m2 = 0)
-      gr[t][0] -= ok ? e0 : zero4;
-      gr[t][1] -= ok ? e1 : zero4;
-      sx0 -= ok ? e0 : zero4;
-      sx1 -= ok ? e1 : zero4;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float e = xr[t][s][i] * m2 + c1, d = ok ? e : 0.f;
+          gr[t][s][i] -= d;
+          sx[s][i] -= d;
+        }
     }
     if (mask_n) {
       const bool okm = (FAST && grp + 2 * t < 12) || p < L;
       const unsigned m8 = okm ? (unsigned)(pm >> (8 * t)) & 255u : 0u;
-      const f32x4 o0 = gr[t][0], o1 = gr[t][1];
       f32x4 v[2];
-      v[0] = f32x4{(m8 & 1u) ? o0[0] : 0.f, (m8 & 2u) ? o0[1] : 0.f, (m8 & 4u) ? o0[2] : 0.f, (m8 & 8u) ? o0[3] : 0.f};
-      v[1] = f32x4{(m8 & 16u) ? o1[0] : 0.f, (m8 & 32u) ? o1[1] : 0.f, (m8 & 64u) ? o1[2] : 0.f, (m8 & 128u) ? o1[3] : 0.f};
-      sc0 += v[0];
-      sc1 += v[1];
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float e = (m8 & (1u << (4 * s + i))) ? gr[t][s][i] : 0.f;
+          v[s][i] = e;
+          sc[s][i] += e;
+        }
       if ((FAST && grp + 2 * t < 12) || p < L) store_h8(smem, p, ch0, v);
     }
   }
@@ -498,8 +515,8 @@ __device__ __forceinline__ void epilogue_lnb(char* smem, f32x4 (&gr)[NT][2], f32
     stat_nx[MAXPOS + tid] = st_r;
   }
   if (part_o) {
-    put_sum(sx0, sx1, 2);
-    put_sum(sc0, sc1, 3);
+    put_sum(quad(sx[0]), quad(sx[1]), 2);
+    put_sum(quad(sc[0]), quad(sc[1]), 3);
   }
   __syncthreads();   // the new dc image and the next statistics are in place
 }
@@ -548,10 +565,10 @@ __device__ __forceinline__ void train_bwd_body(const TrainBwdArgs& a, char* smem
   }
   __syncthreads();
 
-  f32x4 gr[NT][2], acc[NT][2];
+  float gr[NT][2][4] = {};
+  f32x4 acc[NT][2];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    gr[t][0] = gr[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
     acc[t][0] = acc[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   const int lo0 = opaque(lane);
@@ -649,7 +666,7 @@ __device__ __forceinline__ void train_bwd_body(const TrainBwdArgs& a, char* smem
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           const f32x4 f = *(const f32x4*)(f0 + (size_t)(p * 128 + chl + 16 * s));
-          const f32x4 gq = gr[t][s];
+          const float(&gq)[4] = gr[t][s];
           *(f32x4*)(o + (size_t)(p * 128 + chl + 16 * s)) =
               f32x4{f[0] > 0.f ? gq[0] : 0.f, f[1] > 0.f ? gq[1] : 0.f, f[2] > 0.f ? gq[2] : 0.f, f[3] > 0.f ? gq[3] : 0.f};
         }
