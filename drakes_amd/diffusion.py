@@ -28,6 +28,8 @@ from .models import dnaconv
 
 
 class Diffusion(nn.Module):
+    hip_checkpoint = None      # 'int8': the bf16 differentiable path keeps its activations in 8 bits (here for modules stored whole before it was)
+
     def __init__(self, config, eval=False):
         super().__init__()
         if eval:
@@ -50,7 +52,6 @@ class Diffusion(nn.Module):
         self.neg_infinity = -1000000.0
         self.hip_dtype = 'fp32'
         self.hip_soft_dtype = None      # differentiable (Gumbel-softmax) steps: None = follow hip_dtype; 'fp32' | 'bf16'
-        self.hip_checkpoint = None      # 'int8': the bf16 differentiable path keeps its activations in 8 bits
         self.hip_graph = False          # fp32 path: replay the step loop from a captured hipGraph (see _sample_graph)
         self._graph = None
         self._validate_configuration()

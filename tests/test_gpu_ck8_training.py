@@ -264,3 +264,16 @@ def test_gradients_stay_within_a_few_percent_of_the_path_without_checkpoints(dev
     print(f'worst {worst} {rel[worst]:.4f}, median {sorted(rel.values())[len(rel) // 2]:.4f}')
     assert rel[worst] < 0.04, (worst, rel[worst])
     assert sorted(rel.values())[len(rel) // 2] < 0.02
+
+
+@pytest.mark.gpu
+def test_a_model_from_before_the_setting_runs_without_it(dev, det_sd):
+    """A module that was stored whole brings its own attributes along, and hip_checkpoint may not be among them."""
+    m = drakes_amd.Diffusion(drakes_amd.default_config(length=16)).to(dev)
+    m.load_state_dict(det_sd)
+    m.hip_dtype = 'bf16'
+    x = torch.full((2, 16), 4, dtype=torch.int64, device=dev)
+    want = m.score_tokens(x, torch.zeros(1, device=dev), x.clamp(max=3))[0].detach()
+    m.__dict__.pop('hip_checkpoint', None)
+    assert torch.equal(m.score_tokens(x, torch.zeros(1, device=dev), x.clamp(max=3))[0].detach(), want)
+    m.forward(x, torch.zeros(2, device=dev)).sum().backward()
