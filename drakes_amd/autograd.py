@@ -618,7 +618,8 @@ class _BackboneCk8Fn(torch.autograd.Function):
             slabs = (M + 127) // 128
             part = torch.empty(slabs, slab, dtype=torch.float32, device=dev)
             ops.head_bwd_bf16(dlogits, y, pk['head2_w'], dc, partials=part, part_stride=slab)
-            ops.slab_reduce(part, slabs, slab, acc[sink.head_off:], slab)
+            if M:
+                ops.slab_reduce(part, slabs, slab, acc[sink.head_off:], slab)
             ops.conv_wgrad_ck8(kept[n], None, None, dc, dwt[9 * n:], 0)
             if ctx.tb_stride:
                 rows = torch.zeros(n, B, C, dtype=torch.float32, device=dev)

@@ -277,3 +277,29 @@ def test_a_model_from_before_the_setting_runs_without_it(dev, det_sd):
     m.__dict__.pop('hip_checkpoint', None)
     assert torch.equal(m.score_tokens(x, torch.zeros(1, device=dev), x.clamp(max=3))[0].detach(), want)
     m.forward(x, torch.zeros(2, device=dev)).sum().backward()
+
+
+@pytest.mark.parametrize('soft', [False, True])
+def test_an_empty_batch(dev, det_sd, soft):
+    """No rows: empty logits, gradients of zero, as the path without checkpoints gives; alone and as one of a chain."""
+    m = _model(dev, det_sd, length=16, time_conditioning=True)
+    x = torch.empty(0, 16, 5, device=dev, requires_grad=True) if soft else torch.empty(0, 16, dtype=torch.int64, device=dev)
+    out = {}
+    for keep in (None, 'int8'):
+        lg = autograd.backbone_with_grad(m.backbone, x, torch.zeros(1, device=dev), 'bf16', keep=keep)
+        assert lg.shape == (0, 16, 5)
+        lg.sum().backward()
+        out[keep] = _grads(m)
+    assert set(out[None]) == set(out['int8'])
+    assert all(bool((g == 0).all()) for g in out['int8'].values())
+    if soft:
+        assert x.grad.shape == x.shape
+    sink, anchor = autograd.grad_chain(m.backbone)
+    one = torch.randint(0, 5, (2, 16), generator=torch.Generator().manual_seed(1)).to(dev)
+    z = torch.zeros(1, device=dev)
+    both = [autograd.backbone_with_grad(m.backbone, s, z, 'bf16', flat=anchor, sink=sink, sigma_key=0.0, keep='int8') for s in (x, one)]
+    torch.autograd.backward(both, [torch.ones_like(b) for b in both])
+    got = _grads(m)
+    autograd.backbone_with_grad(m.backbone, one, z, 'bf16', keep='int8').sum().backward()
+    for k, g in _grads(m).items():
+        assert float((g - got[k]).norm()) <= 1e-5 * float(g.norm()) + 1e-7, k
