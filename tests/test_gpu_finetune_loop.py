@@ -164,3 +164,34 @@ def test_kl_side_streams_change_nothing(dev, det_sd, dtype):
         g2 = res[2][1][k]
         scale = float(g0.abs().max()) + 1e-12
         assert float((g0 - g2).abs().max()) <= 1e-5 * scale, (k, float((g0 - g2).abs().max()) / scale)
+
+
+def test_kl_side_streams_change_nothing_with_8_bit_activations(dev, det_sd):
+    """hip_checkpoint = 'int8' on the new model and on the frozen one, whose forwards and input gradients run on side streams;
+    and the frozen model's own setting decides what it keeps."""
+    args = NS(truncate_steps=4, gumbel_temp=1.0, total_num_steps=12, learning_rate=1e-4, num_epochs=1, num_accum_steps=2,
+              batch_size=3, copy_flag_temp=None, truncate_kl=False, alpha=0.01, alpha_schedule_warmup=0, gradnorm_clip=1.0,
+              name='debug', save_every_n_epochs=10 ** 9)
+    res = {}
+    for ks, old_keep in ((0, 'int8'), (2, 'int8'), (2, None)):
+        new_model = drakes_amd.Diffusion(drakes_amd.default_config(steps=12)).to(dev)
+        old_model = drakes_amd.Diffusion(drakes_amd.default_config(steps=12)).to(dev)
+        new_model.load_state_dict(det_sd)
+        old_model.load_state_dict({k: v + 0.01 for k, v in det_sd.items()})
+        new_model.hip_dtype = old_model.hip_dtype = 'bf16'
+        new_model.hip_checkpoint, old_model.hip_checkpoint = 'int8', old_keep
+        first = {}
+
+        def grab(model, epoch):
+            first.update({k: p.grad.detach().cpu().clone() for k, p in model.named_parameters() if p.grad is not None})
+        losses = drakes_amd.fine_tune(new_model, SyntheticReward(3).to(dev), SyntheticReward(4).to(dev), old_model, args,
+                                      seed_of_call=lambda i: 50 + i, verbose=False, on_update=grab, kl_streams=ks)
+        assert new_model.backbone.train_keep == 'int8' and old_model.backbone.train_keep == old_keep
+        res[ks, old_keep] = ([float(x) for x in losses], first)
+    (la, ga), (lb, gb) = res[0, 'int8'], res[2, 'int8']
+    np.testing.assert_allclose(la, lb, rtol=1e-6, atol=1e-7)
+    for k, g0 in ga.items():                                 # (the stem's and the time path's sums use atomics)
+        scale = float(g0.abs().max()) + 1e-12
+        assert float((g0 - gb[k]).abs().max()) <= 1e-5 * scale, k
+    # a frozen model with full activations: its forward's bf16 roundings and the 8 bits of its input gradient only
+    np.testing.assert_allclose(la, res[2, None][0], rtol=2e-2, atol=2e-3)
