@@ -48,15 +48,15 @@ PEAK = {'bf16': 2500.0, 'fp32': 157.3}            # TFLOP/s dense MFMA, MI355X_M
 # for 16-B-per-lane loads on gfx950): tools/pmc_traffic.sh.  A recorded measurement (a process cannot collect PMC
 # counters on itself): it names the library version it was taken on and is printed ONLY when drk_version() still is
 # that version — a changed kernel reports traffic null until the passes are re-run.
-PMC_TRAFFIC = {('bf16', 1024): {'drk_version': 312,
-                                'bytes_per_launch': 26807637248.0, 'fetch_bytes': 26225558400.0, 'write_bytes': 582078848.0,
+PMC_TRAFFIC = {('bf16', 1024): {'drk_version': 313,
+                                'bytes_per_launch': 26806081280.0, 'fetch_bytes': 26224107392.0, 'write_bytes': 581973888.0,
                                 'algorithmic_bytes': 7.6e6,
                                 'note': 'L2-to-fabric requests; Infinity-Cache hits are counted: the 5.9 MB bf16 weight '
                                         'stream outgrows a 4 MB per-XCD L2 and is re-fetched from the 256 MB Infinity '
                                         'Cache; 0.24 TB/s = 3.0 % of HBM peak, the launch is MFMA-bound; the writes are '
-                                        'scratch spills of the per-forward stem/head block (140 B/lane reserved; 2 dwords per lane and forward '
-                                        'actually written), tokens out are 1.6 MB',
-                                'source': 'profiles/bf16_v312_pmc_traffic.json'}}
+                                        'scratch spills of the per-forward stem/head block (140 B/lane reserved, 8.6 B written per lane and '
+                                        'forward), tokens out are 1.6 MB',
+                                'source': 'profiles/bf16_v313_pmc_traffic.json'}}
 
 
 def _median(v):
@@ -263,8 +263,8 @@ def secondary_fp32(model, B=1024, dtype='fp32'):
 
 
 # The dominant launch of configs[4] (k_group_bf16<8,true>: layers 8..19 + head, B=256, L=1024): tools/pmc_group.sh,
-# profiles/group_v312_pmc.json.  Printed only while drk_version() is the version it was taken on.
-PMC_TRAFFIC_LONG = {'drk_version': 312, 'bytes_per_launch': 383245184.0, 'fetch_bytes': 303397888.0, 'write_bytes': 79847296.0,
+# profiles/group_v313_pmc.json.  Printed only while drk_version() is the version it was taken on.
+PMC_TRAFFIC_LONG = {'drk_version': 313, 'bytes_per_launch': 384164096.0, 'fetch_bytes': 303397888.0, 'write_bytes': 80766208.0,
                     'launch': 'the largest of the three: layers 8..19 + head, stride 4 (the two halo launches: 360 MB each)',
                     'algorithmic_bytes': 256 * 1024 * (512 + 20.0),
                     'note': 'L2-to-fabric requests (FETCH_SIZE doubled per MI355X_MICROARCH.md); beyond the 134 MB of residual '

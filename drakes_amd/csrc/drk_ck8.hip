@@ -317,12 +317,14 @@ __global__ void __launch_bounds__(256) k_ck8_sums(const float* __restrict__ slab
 //     read and decoded once per chunk whatever the number of taps (decoded per tap, the vector instructions alone took
 //     longer than the product).  8 waves, each four taps x 16 ci x 64 co, half of tap 8 and a quarter of S: 76 accumulator
 //     registers, 9 fragments for 19 matrix instructions, the next step's fragments requested among this step's product.
-//     262 144 rows, 9 taps: 84 to 101 us by dilation, and 9 us for the join (95 to 110 us together, 700 to 810 TFLOP/s).
-//     The matrix instructions alone take 46 us of that at the clock they leave the chip; the rest is their waiting for
-//     fragments from LDS, for the staging of tiles and, where sequences end inside a step, for the masks.
+//     262 144 rows, 9 taps, with the join: sequences of 1 024 83 to 99 us by dilation, of 200 94 to 124 us, where more
+//     steps have rows that leave their sequence (all at dilation 64) and taps are multiplied whether they reach a row or not.
+//     The matrix instructions of a step take 608 cycles of a SIMD (2 waves x 19 x 16), its fragments 74 KB of LDS reads, 576
+//     cycles at 128 bytes a cycle: both are full at once, and only fewer fragments per product would change that.  Masks, the
+//     staging of tiles and the join (9 us) are the rest.
 //   k_wgrad_ck8_tap: one tap and 64 input channels per workgroup, for one tap, for few rows (nine times the workgroups per
 //     row chunk, and every chunk costs a slab of P written and read) and for shifts that no ring in LDS can hold
-//     ((taps - 1) * dilation > 832).  262 144 rows: one tap 41 us, 9 taps 290 to 300 us.
+//     ((taps - 1) * dilation > 832).  262 144 rows, with the join: one tap 38 us, 9 taps of dilation 128 208 us.
 #define CW_TILE 64
 #define CW_DC (CW_TILE * 256)            // bytes of a dc tile
 #define CW_SLAB ((DRK_C + 1) * DRK_C)    // P [128][128], then S [128]
@@ -837,8 +839,17 @@ extern "C" int drk_ln_bwd_ck8(const float* dh, const signed char* codes, const u
 // How the work is cut.  All taps in one workgroup (the ring) or one tap per workgroup; row chunks so that every CU has one
 // workgroup of the ring kernel or two of the other, no more, because every chunk costs a slab of P and S per tap written and
 // read (half as many workgroups: 155 us instead of 99 at 262 144 rows; one tap, one against two: 50 and 40 us).
-// From this many rows on the ring is the faster one (9 taps of dilation 1 to 16, 128 channels; ring against one tap per
-// workgroup: 6 400 rows 27 and 23 us, 12 800 rows 30 and 30, 25 600 rows 31 and 43, 262 144 rows 99 and 298).
+// From this many rows on the ring is the faster one.  Ring against one tap per workgroup, us, sequences of 200:
+//                     6 400        12 800        25 600       102 400       262 000 rows
+//   9 taps, d = 4   25.9  22.4    28.0  29.3    29.3  40.8    50.0 112.2    97.0 267.9
+//   9 taps, d = 64  26.8  20.1    29.8  24.9    32.3  33.3    61.1  84.0   123.9 196.0
+//   7 taps, d = 1   22.6  21.5    24.6  26.6    26.5  36.1    44.9  89.4    90.3 210.8
+//   5 taps, d = 1   20.6  20.5    22.6  23.2    24.6  29.3    42.2  67.2    87.2 153.6
+//   3 taps, d = 1   17.3  16.1    20.1  17.8    22.3  21.3    39.8  43.9    84.5  97.8
+//   3 taps, d = 64  17.7  15.8    21.6  17.5    25.0  21.2    48.0  42.2   104.3  92.8
+// (sequences of 1 024: the same within a tenth at d = 1 to 16, and the ring gains at d = 64: 100 and 238 at 262 144 rows.)  The
+// rule is the model's own, nine taps; at three, and near the border at wide dilations, it gives up to 5 us away (12 us, a
+// tenth, at three taps of dilation 64).
 #define CW_RING_ROWS 12800
 struct CwPlan {
   bool ring;

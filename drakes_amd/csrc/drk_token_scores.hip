@@ -12,10 +12,10 @@
 // held at -1e29, so that the product is 0 and not NaN: 2^30 of them do not overflow, and up to T = 1e26 the exponential of
 // anything below it is 0.  From T = 1e-38 on log2(e) / T is a number.  A NaN or +inf among A makes s, logp and H NaN.
 //
-// A forward pass reads every logit once (the bound: HBM), a backward pass reads them again and writes as much.  Kernel
-// times, forward + backward: 204 800 x 5 fp32 5.2 + 5.4 us; 4 080 x 1 001 fp16, masked, 4 alternatives 10.8 + 9.0 us;
-// 2 049 x 50 021 bf16 57 + 74 us (205 and 410 MB: 3.6 and 5.5 TB/s); forward 3 x 131 072 bf16 with 8 alternatives 9.5 + 6.6
-// us (split and join).  Up to some thousand rows of this a call is bound by its launches.  Three
+// A forward pass reads every logit once, a backward pass reads them again and writes as much.  Kernel times, forward +
+// backward: 204 800 x 5 fp32 5.2 + 5.5 us; 4 080 x 1 001 fp16, masked, 4 alternatives 10.7 + 9.4 us; 2 049 x 50 021 bf16 58 +
+// 75 us (205 and 410 MB: 3.5 and 5.5 TB/s; the forward takes 41 us where the Infinity Cache holds the logits: its vector work,
+// which hides the reads from HBM only in part); forward 3 x 131 072 bf16 with 8 alternatives 9.1 + 6.7 us (split and join).  Up to some thousand rows of this a call is bound by its launches.  Three
 // shapes of work, chosen by V and the number of rows alone:
 //   V <= 64        one thread per row; 64 rows at a time come through LDS, so that short rows are still read and written as
 //                  whole cache lines (k_scores_small, k_scores_small_bwd);

@@ -16,8 +16,8 @@ Differences a caller can see, all additive:
     the convolutions at fp32 grade on the bf16 matrix cores (three bf16 planes per operand: logits within ~1e-5 of the
     exact path's, ~3x its speed; under autograd the forward and input-gradient convolutions use it, weight gradients stay
     on the f32 MFMA), or the bf16-MFMA fast path (one launch per `_sample`; differentiable steps on the bf16 layer kernels);
-    `hip_checkpoint = 'int8'` keeps the bf16 differentiable path's activations in 8 bits (a quarter of the memory, and
-    gradients within about a percent); `hip_graph = True` replays the fp32 step loop from a captured hipGraph.
+    `hip_checkpoint = 'int8'` keeps the bf16 differentiable path's activations in 8 bits (a fifth of the memory, and
+    gradients within one to a few percent); `hip_graph = True` replays the fp32 step loop from a captured hipGraph.
 """
 import torch
 import torch.nn as nn

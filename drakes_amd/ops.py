@@ -672,10 +672,11 @@ def _score_args(name, logits, tokens, allowed, temp):
     kind = _SCORE_TYPES.get(logits.dtype)
     if kind is None:
         raise TypeError(f'{name}: logits are float32, bfloat16 or float16, got {logits.dtype}')
-    if logits.ndim < 1 or logits.shape[-1] < 1 or tokens.shape != logits.shape[:-1]:
-        raise ValueError(f'{name}: logits [..., V] and tokens [...], got {tuple(logits.shape)} and {tuple(tokens.shape)}')
-    if logits.shape[-1] > V_MAX:               # (V and the columns' numbers are 32-bit: a larger one would wrap on the way)
-        raise ValueError(f'{name}: at most 2^30 columns, got {logits.shape[-1]}')
+    shape = logits.shape
+    if not shape or shape[-1] < 1 or tokens.shape != shape[:-1]:
+        raise ValueError(f'{name}: logits [..., V] and tokens [...], got {tuple(shape)} and {tuple(tokens.shape)}')
+    if shape[-1] > V_MAX:                      # (V and the columns' numbers are 32-bit: a larger one would wrap on the way)
+        raise ValueError(f'{name}: at most 2^30 columns, got {shape[-1]}')
     if not TEMP_MIN <= temp <= TEMP_MAX:
         raise ValueError(f'{name}: temp must be in [{TEMP_MIN}, {TEMP_MAX}], got {temp}')
     dev, stream = _current()
@@ -685,11 +686,11 @@ def _score_args(name, logits, tokens, allowed, temp):
     if allowed is not None:
         if allowed.dtype is not torch.bool and allowed.dtype is not torch.uint8:
             raise TypeError(f'{name}: allowed is bool or uint8, got {allowed.dtype}')
-        if allowed.shape != logits.shape[-1:] and allowed.shape != logits.shape:
+        if allowed.shape != shape[-1:] and allowed.shape != shape:
             raise ValueError(f'{name}: allowed has shape [V] or that of the logits, got {tuple(allowed.shape)}')
         al = _at(allowed, allowed.dtype, 'allowed', dev)
         if allowed.ndim > 1:
-            al_stride = logits.shape[-1]
+            al_stride = shape[-1]
     return dev, stream, (logits.data_ptr(), kind, _row_stride(logits, name), _at(tokens, torch.int64, 'tokens', dev), al, al_stride,
                          temp)
 
