@@ -136,7 +136,8 @@ long drk_token_scores_workspace_bytes(long rows, int V, int dtype);
 /* Gradient of sum g_logp logp + sum g_entropy entropy + sum g_top top_logp with respect to the logits (each g optional;
  * g_logp needs the logp, g_entropy the entropy, g_top the ids that the forward gave, else k = 0).  dlogits [rows][V], dense, of the logits'
  * type, every element written: 0 in columns that do not count; it may be the logits themselves when they are dense.  A log-probability of -inf, 0 (not scored) or NaN (token
- * >= V) passes no gradient, nor does a place with id -1. */
+ * >= V) passes no gradient, nor does a place with id -1.  A row into which no gradient comes (every g 0 or not passed on) is 0
+ * whatever its logits hold; in one with a NaN or +inf and a gradient, the columns that count are NaN. */
 int drk_token_scores_bwd(const void* logits, int dtype, long row_stride, const int64_t* tokens, const unsigned char* allowed,
                          long allowed_stride, float temp, int k, const float* stats, const float* logp, const float* entropy,
                          const int64_t* top_ids, const float* g_logp, const float* g_entropy, const float* g_top,
